@@ -97,6 +97,53 @@ void mxfp6_gemm_gather(int ot, int M, int N, int Kp, const void* dA, const void*
                        const uint8_t* dsB, void* const* dDs, int n_dst, long long ldd, int col0, int A_row_bytes,
                        int B_row_bytes, void* ws, size_t ws_bytes, void* stream);
 
+/* ---- fused epilogue ------------------------------------------------------------------------
+ * No counterpart in the reference, whose GEMM writes D = A·B and leaves the rest of a layer to
+ * further kernels. */
+
+/* Activations: v, max(v, 0), v*Phi(v) with the error function, its tanh form
+ * 0.5 v (1 + tanh(sqrt(2/pi) (v + 0.044715 v^3))), and v / (1 + e^-v). */
+enum mxfp6_activation {
+    MXFP6_ACT_NONE = 0, MXFP6_ACT_RELU = 1, MXFP6_ACT_GELU = 2, MXFP6_ACT_GELU_TANH = 3, MXFP6_ACT_SILU = 4
+};
+/* How the aux operand joins: not at all, added (a residual), or multiplied (a gate's other half). */
+enum mxfp6_aux_op { MXFP6_AUX_NONE = 0, MXFP6_AUX_ADD = 1, MXFP6_AUX_MUL = 2 };
+
+typedef struct mxfp6_epilogue {
+    const void* bias;   /* [N], or NULL */
+    const void* aux;    /* [M][ld_aux]; read when aux_op is not MXFP6_AUX_NONE */
+    long long ld_aux;   /* elements between aux rows, >= N */
+    int bias_type;      /* enum mxfp6_out_type */
+    int activation;     /* enum mxfp6_activation */
+    int aux_op;         /* enum mxfp6_aux_op */
+    int aux_type;       /* enum mxfp6_out_type */
+} mxfp6_epilogue;
+
+/* D = op(act(A·B + bias), aux), computed on the FP32 accumulator and rounded once to D's type.
+ * A NULL epilogue is D = A·B. Operands as for mxfp6_gemm_stream, but any M >= 0 (0 launches nothing)
+ * and any N > 0: no operand is padded, and the tiled scales have the size mxfp6_tiled_scale_bytes
+ * gives. D is row-major with ldd >= N elements between rows; D, bias and aux need only the alignment
+ * of their elements (16-byte aligned rows take wide accesses). D may be the aux operand itself (same
+ * address, pitch and type); otherwise the two do not overlap. Rows and columns outside [M][N] are
+ * not written. The workspace contract is mxfp6_gemm's, with mxfp6_gemm_fused_workspace_size. Returns
+ * an mxfp6_status, which mxfp6_last_error() also reports. */
+int mxfp6_gemm_fused(int ot, int M, int N, int Kp, const void* dA, const void* dBsh, const uint8_t* dsA,
+                     const uint8_t* dsB, void* dD, long long ldd, int A_row_bytes, int B_row_bytes,
+                     const mxfp6_epilogue* epilogue, void* ws, size_t ws_bytes, void* stream);
+
+/* The same with D quantised to MXFP6 as by mxfp6_quantize_device_padded (N % 128 == 0): packed rows
+ * of packed_row_bytes (>= 3N/4, a multiple of 32; 32-byte aligned base) and tiled scales (16-byte
+ * aligned), which are the A operand of a following GEMM with Kp = N. Scales of rows past M in the
+ * last atom are not written. */
+int mxfp6_gemm_fused_quant(int M, int N, int Kp, const void* dA, const void* dBsh, const uint8_t* dsA,
+                           const uint8_t* dsB, uint8_t* d_packed, int packed_row_bytes, uint8_t* d_scales,
+                           int A_row_bytes, int B_row_bytes, const mxfp6_epilogue* epilogue, void* ws,
+                           size_t ws_bytes, void* stream);
+
+/* Workspace bytes the two fused calls use (any output type), with room for a padded copy of A when
+ * A_row_bytes is a stride the tensor load cannot address. */
+size_t mxfp6_gemm_fused_workspace_size(int M, int N, int Kp, int A_row_bytes);
+
 /* CUDA IPC for mxfp6_gemm_gather's peer destinations. export: a 64-byte handle of the
  * allocation holding dptr, and dptr's offset in it. import (in another process, with its own
  * device current): maps the allocation, returns its base (for close) and the pointer. */
@@ -241,6 +288,13 @@ int mxfp6_quantize_device(const float* d_mat, int rows, int cols, uint8_t* d_pac
  * No counterpart in the reference, whose "compact A" recipe reads rows of K codes in place. */
 int mxfp6_quantize_device_padded(const float* d_mat, int rows, int cols, int padded_cols, uint8_t* d_packed,
                                  uint8_t* d_scales, int scale_layout, void* stream);
+
+/* The same for an input of any type (in_type: enum mxfp6_out_type; FP16 and BF16 are exact in FP32, so
+ * the result is that of quantising the FP32 values) with ld >= cols elements between rows, aligned to
+ * its elements (16-byte aligned rows take wide loads), and any number of rows (0 launches nothing). No
+ * counterpart in the reference. */
+int mxfp6_quantize_device_typed(const void* d_mat, int in_type, int rows, int cols, long long ld, int padded_cols,
+                                uint8_t* d_packed, uint8_t* d_scales, int scale_layout, void* stream);
 
 /* dequantize_mxfp6 (reference: include/mxfp6/preprocess.hpp:100-109). */
 void mxfp6_dequantize(const uint8_t* packed, const uint8_t* scales, int rows, int cols,

@@ -284,6 +284,10 @@ int a_mode(int Kp, const void* dA, int A_row_bytes) {
     return a_uses_tma(Kp, dA, A_row_bytes) ? kern::A_TMA : kern::A_CPASYNC;
 }
 
+// Operand strides, pointers and their alignment (the output's is checked by the caller).
+bool validate_operands(int Kp, const void* dA, const void* dB, const void* sA, const void* sB, const void* dD,
+                       int A_row_bytes, int B_row_bytes);
+
 bool validate(int ot, int M, int N, int Kp, const void* dA, const void* dB, const void* sA,
               const void* sB, const void* dD, int A_row_bytes, int B_row_bytes) {
     if (ot < MXFP6_OUT_F32 || ot > MXFP6_OUT_BF16) {
@@ -297,6 +301,16 @@ bool validate(int ot, int M, int N, int Kp, const void* dA, const void* dB, cons
                   M, N, Kp, K_TILE);
         return false;
     }
+    if (!validate_operands(Kp, dA, dB, sA, sB, dD, A_row_bytes, B_row_bytes)) return false;
+    if (!aligned(dD, 16)) {
+        set_error(MXFP6_ERR_MISALIGNED, "misaligned pointer: D needs 16-byte alignment");
+        return false;
+    }
+    return true;
+}
+
+bool validate_operands(int Kp, const void* dA, const void* dB, const void* sA, const void* sB, const void* dD,
+                       int A_row_bytes, int B_row_bytes) {
     const long long need = (long long)Kp * 3 / 4;
     if (B_row_bytes < need || B_row_bytes % 32) {
         set_error(MXFP6_ERR_INVALID_STRIDE,
@@ -317,12 +331,69 @@ bool validate(int ot, int M, int N, int Kp, const void* dA, const void* dB, cons
                   sA, sB, dD);
         return false;
     }
-    if (!aligned(dA, 4) || !aligned(dB, 32) || !aligned(sA, 16) || !aligned(sB, 16) || !aligned(dD, 16)) {
+    if (!aligned(dA, 4) || !aligned(dB, 32) || !aligned(sA, 16) || !aligned(sB, 16)) {
         set_error(MXFP6_ERR_MISALIGNED,
                   "misaligned pointer: A needs 4-byte (32-byte for the tensor-load path), B 32-byte, "
-                  "scales and D 16-byte alignment");
+                  "scales 16-byte alignment");
         return false;
     }
+    return true;
+}
+
+int type_bytes(int type) {
+    return type == MXFP6_OUT_F32 ? 4 : 2;
+}
+bool valid_type(int type) {
+    return type >= MXFP6_OUT_F32 && type <= MXFP6_OUT_BF16;
+}
+
+// Checks a caller's epilogue description for an N-column output and fills the kernels' form of it
+// (all but the output).
+bool validate_epilogue(const mxfp6_epilogue* ep, int M, int N, kern::Epi& e) {
+    std::memset(&e, 0, sizeof(e));
+    if (!ep) return true;
+    if (ep->activation < MXFP6_ACT_NONE || ep->activation > MXFP6_ACT_SILU || ep->aux_op < MXFP6_AUX_NONE ||
+        ep->aux_op > MXFP6_AUX_MUL) {
+        set_error(MXFP6_ERR_UNSUPPORTED, "epilogue: activation %d, aux operation %d", ep->activation, ep->aux_op);
+        return false;
+    }
+    if (ep->bias) {
+        if (!valid_type(ep->bias_type)) {
+            set_error(MXFP6_ERR_INVALID_OUT_TYPE, "epilogue: invalid bias type %d", ep->bias_type);
+            return false;
+        }
+        if (!aligned(ep->bias, type_bytes(ep->bias_type))) {
+            set_error(MXFP6_ERR_MISALIGNED, "epilogue: the bias is not aligned to its element");
+            return false;
+        }
+    }
+    if (ep->aux_op != MXFP6_AUX_NONE) {
+        if (!valid_type(ep->aux_type)) {
+            set_error(MXFP6_ERR_INVALID_OUT_TYPE, "epilogue: invalid aux type %d", ep->aux_type);
+            return false;
+        }
+        if (!ep->aux) {
+            set_error(MXFP6_ERR_NULL_POINTER, "epilogue: aux operation %d without an aux operand", ep->aux_op);
+            return false;
+        }
+        if (!aligned(ep->aux, type_bytes(ep->aux_type))) {
+            set_error(MXFP6_ERR_MISALIGNED, "epilogue: the aux operand is not aligned to its element");
+            return false;
+        }
+        if (ep->ld_aux < N && M > 1) {
+            set_error(MXFP6_ERR_INVALID_STRIDE, "epilogue: aux pitch %lld is below N = %d", ep->ld_aux, N);
+            return false;
+        }
+        e.aux = ep->aux;
+        e.ld_aux = ep->ld_aux;
+        e.aux_type = ep->aux_type;
+        e.aux_op = ep->aux_op;
+        e.aux_vec = aligned(ep->aux, 16) && (M <= 1 || ep->ld_aux * type_bytes(ep->aux_type) % 16 == 0);
+    }
+    e.bias = ep->bias;
+    e.bias_type = ep->bias_type;
+    e.bias_vec = aligned(ep->bias, 16);
+    e.act = ep->activation;
     return true;
 }
 
@@ -351,10 +422,27 @@ void set_pdl(cudaLaunchAttribute& a) {
     a.val.programmaticStreamSerializationAllowed = 1;
 }
 
+// A launch with a fused epilogue: its parameters, and the rows B really has. A split launch (PARTIAL)
+// then runs with N rounded up to 32, the pitch of its partials, and takes only `n_rows` from here.
+struct FusedLaunch {
+    kern::Epi epi;
+    int n_rows;
+};
+
+template <typename OutT, bool PARTIAL>
+int out_align32(const float* ws, const kern::DstList& dl) {
+    if constexpr (PARTIAL)
+        return aligned(ws, 32) ? 1 : 0;
+    else if constexpr (std::is_same<OutT, kern::FusedOut>::value)
+        return 0;  // the fused epilogue keeps its own alignment flags
+    else
+        return dst_align32(dl, sizeof(OutT)) ? 1 : 0;
+}
+
 template <int BN, typename OutT, bool PARTIAL, int AMODE>
 bool launch_gemm(int M, int N, int Kp, const void* dA, const void* dB, const uint8_t* sA,
                  const uint8_t* sB, const kern::DstList& dl, float* ws, int A_row_bytes, int B_row_bytes,
-                 int splits, cudaStream_t stream) {
+                 int splits, cudaStream_t stream, const FusedLaunch* fused = nullptr) {
     using C = kern::Config<BN, AMODE>;
     auto kernel = kern::gemm_mxfp6_sm100<BN, OutT, PARTIAL, AMODE>;
     static std::once_flag attr_once[kMaxDevices];
@@ -373,12 +461,13 @@ bool launch_gemm(int M, int N, int Kp, const void* dA, const void* dB, const uin
     }
     CUtensorMap tmA, tmB;
     if (!make_a_tmap(AMODE, &tmA, dA, M, Kp, A_row_bytes, kern::BM) ||
-        !make_fp6_tmap(&tmB, dB, N, Kp, B_row_bytes, BN)) {
+        !make_fp6_tmap(&tmB, dB, fused ? fused->n_rows : N, Kp, B_row_bytes, BN)) {
         set_error(MXFP6_ERR_CUDA, "cuTensorMapEncodeTiled failed for %dx%dx%d (status %d)", M, N, Kp,
                   t_encode_status);
         return false;
     }
-    kern::Params p;
+    kern::ParamsFor<OutT> p;
+    if constexpr (std::is_same<OutT, kern::FusedOut>::value) p.epi = fused->epi;
     p.sfA = sA;
     p.sfB = sB;
     p.dst = dl;
@@ -386,11 +475,11 @@ bool launch_gemm(int M, int N, int Kp, const void* dA, const void* dB, const uin
     p.M = M;
     p.N = N;
     p.Kp = Kp;
-    p.m_blocks = M / kern::BM;
+    p.m_blocks = (M + kern::BM - 1) / kern::BM;
     p.n_blocks = (N + BN - 1) / BN;
     p.k_slabs = Kp / kern::BK;
     p.splits = splits;
-    p.out_align32 = (PARTIAL ? aligned(ws, 32) : dst_align32(dl, sizeof(OutT))) ? 1 : 0;
+    p.out_align32 = out_align32<OutT, PARTIAL>(ws, dl);
     set_compact(p, Kp, dA, A_row_bytes);
     p.wait_budget = wait_budget();
     const long long tiles = (long long)p.m_blocks * p.n_blocks * splits;
@@ -423,13 +512,15 @@ bool launch_gemm(int M, int N, int Kp, const void* dA, const void* dB, const uin
 template <typename OutT, bool PARTIAL, int AMODE>
 bool launch_pair(int M, int N, int Kp, const void* dA, const void* dB, const uint8_t* sA, const uint8_t* sB,
                  const kern::DstList& dl, float* ws, int A_row_bytes, int B_row_bytes, int splits, void* sk_area,
-                 cudaStream_t stream, const BandedSplit* band = nullptr) {
+                 cudaStream_t stream, const BandedSplit* band = nullptr, const FusedLaunch* fused = nullptr) {
     using C = kern::PairConfig<AMODE>;
     // the kernel without stream-K hand-offs and multi-destination stores, with hand-offs, and with
     // both (one instantiation in partial mode, which has neither)
     auto kernel_lean = kern::gemm_mxfp6_sm100_pair<OutT, PARTIAL, AMODE, kern::EPI_LEAN>;
     auto kernel_sk = kern::gemm_mxfp6_sm100_pair<OutT, PARTIAL, AMODE, PARTIAL ? kern::EPI_LEAN : kern::EPI_STREAM_K>;
-    auto kernel_all = kern::gemm_mxfp6_sm100_pair<OutT, PARTIAL, AMODE, PARTIAL ? kern::EPI_LEAN : kern::EPI_ALL>;
+    constexpr bool FUSED = std::is_same<OutT, kern::FusedOut>::value;  // one destination, always
+    auto kernel_all = kern::gemm_mxfp6_sm100_pair<OutT, PARTIAL, AMODE,
+                                                  PARTIAL ? kern::EPI_LEAN : FUSED ? kern::EPI_STREAM_K : kern::EPI_ALL>;
     static std::once_flag attr_once[kMaxDevices];
     const int dev = current_device();
     if (dev < 0 || dev >= kMaxDevices) {
@@ -453,13 +544,14 @@ bool launch_pair(int M, int N, int Kp, const void* dA, const void* dB, const uin
     const bool banded = PARTIAL && band && band->L > 0;
     const int clusters = banded ? pairs : (int)(tiles < pairs ? tiles : pairs);
     CUtensorMap tmA, tmB, tmSA, tmSB;
-    if (!make_a_tmap(AMODE, &tmA, dA, M, Kp, A_row_bytes, 128) || !make_fp6_tmap(&tmB, dB, N, Kp, B_row_bytes, 128) ||
+    if (!make_a_tmap(AMODE, &tmA, dA, M, Kp, A_row_bytes, 128) || !make_fp6_tmap(&tmB, dB, fused ? fused->n_rows : N, Kp, B_row_bytes, 128) ||
         !make_sf_tmap(&tmSA, sA, M, Kp, 1, C::SUB) || !make_sf_tmap_x4(&tmSB, sB, N, Kp)) {
         set_error(MXFP6_ERR_CUDA, "cuTensorMapEncodeTiled failed for %dx%dx%d (status %d)", M, N, Kp,
                   t_encode_status);
         return false;
     }
-    kern::Params p;
+    kern::ParamsFor<OutT> p;
+    if constexpr (FUSED) p.epi = fused->epi;
     p.sfA = sA;
     p.sfB = sB;
     p.dst = dl;
@@ -471,7 +563,7 @@ bool launch_pair(int M, int N, int Kp, const void* dA, const void* dB, const uin
     p.n_blocks = n_blocks;
     p.k_slabs = Kp / kern::BK;
     p.splits = splits;
-    p.out_align32 = (PARTIAL ? aligned(ws, 32) : dst_align32(dl, sizeof(OutT))) ? 1 : 0;
+    p.out_align32 = out_align32<OutT, PARTIAL>(ws, dl);
     set_compact(p, Kp, dA, A_row_bytes);
     p.wait_budget = wait_budget();
     // Stream-K tail (sk_area non-null, laid out as stream_k_bytes(clusters)): the last waves'
@@ -541,13 +633,44 @@ bool launch_reduce(const float* ws, const kern::DstList& dl, int M, int N, int s
     return true;
 }
 
+bool launch_reduce_fused(const float* ws, const kern::Epi& epi, int M, int N, int Np, int splits, cudaStream_t stream) {
+    const long long n4 = (long long)M * Np / 4;
+    long long blocks = (n4 + 255) / 256;
+    const long long cap = (long long)sm_count() * 8;
+    if (blocks > cap) blocks = cap;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)blocks, 1, 1);
+    cfg.blockDim = dim3(256, 1, 1);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    set_pdl(attr[0]);
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kern::reduce_partials_fused, ws, epi, M, N, Np, splits);
+    if (e == cudaSuccess) e = cudaGetLastError();
+    if (e != cudaSuccess) {
+        set_error(MXFP6_ERR_CUDA, "fused split-K reduce launch failed: %s", cudaGetErrorString(e));
+        return false;
+    }
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+    return true;
+}
+
+// Columns of a fused launch's split-K partials: whole 32-column chunks.
+int partials_pitch(int N) {
+    return (N + 31) / 32 * 32;
+}
+
 // Partial (split-K) launches write FP32 whatever the output type, so they share the float
 // instantiation; the reduce pass converts.
 template <typename OutT, int AMODE>
 bool run_route(const Route& r, int M, int N, int Kp, const void* dA, const void* dB, const uint8_t* sA,
-               const uint8_t* sB, const kern::DstList& dl, int Ar, int Br, void* ws, cudaStream_t stream) {
+               const uint8_t* sB, const kern::DstList& dl, int Ar, int Br, void* ws, cudaStream_t stream,
+               const FusedLaunch* fused = nullptr) {
     float* wsf = static_cast<float*>(ws);
     const bool part = r.splits > 1;
+    const int n_real = N;
+    if (fused && part) N = partials_pitch(N);
     bool ok;
     if (r.MT == 256) {
         // the stream-K hand-off area follows the split-K partials in the workspace
@@ -559,18 +682,23 @@ bool run_route(const Route& r, int M, int N, int Kp, const void* dA, const void*
             band = banded_split(tiles, sm_count() / 2, Kp / K_TILE, r.splits - L);
         }
         ok = part ? launch_pair<float, true, AMODE>(M, N, Kp, dA, dB, sA, sB, dl, wsf, Ar, Br, r.splits, nullptr,
-                                                    stream, r.banded ? &band : nullptr)
-                  : launch_pair<OutT, false, AMODE>(M, N, Kp, dA, dB, sA, sB, dl, wsf, Ar, Br, 1, sk, stream);
+                                                    stream, r.banded ? &band : nullptr, fused)
+                  : launch_pair<OutT, false, AMODE>(M, N, Kp, dA, dB, sA, sB, dl, wsf, Ar, Br, 1, sk, stream, nullptr,
+                                                    fused);
     } else if (r.NT == 256) {
         ok = part ? launch_gemm<256, float, true, AMODE>(M, N, Kp, dA, dB, sA, sB, dl, wsf, Ar, Br, r.splits,
-                                                           stream)
-                  : launch_gemm<256, OutT, false, AMODE>(M, N, Kp, dA, dB, sA, sB, dl, wsf, Ar, Br, 1, stream);
+                                                           stream, fused)
+                  : launch_gemm<256, OutT, false, AMODE>(M, N, Kp, dA, dB, sA, sB, dl, wsf, Ar, Br, 1, stream, fused);
     } else {
         ok = part ? launch_gemm<128, float, true, AMODE>(M, N, Kp, dA, dB, sA, sB, dl, wsf, Ar, Br, r.splits,
-                                                           stream)
-                  : launch_gemm<128, OutT, false, AMODE>(M, N, Kp, dA, dB, sA, sB, dl, wsf, Ar, Br, 1, stream);
+                                                           stream, fused)
+                  : launch_gemm<128, OutT, false, AMODE>(M, N, Kp, dA, dB, sA, sB, dl, wsf, Ar, Br, 1, stream, fused);
     }
-    return ok && (!part || launch_reduce<OutT>(wsf, dl, M, N, r.splits, stream));
+    if (!ok || !part) return ok;
+    if constexpr (std::is_same<OutT, kern::FusedOut>::value)
+        return launch_reduce_fused(wsf, fused->epi, M, n_real, N, r.splits, stream);
+    else
+        return launch_reduce<OutT>(wsf, dl, M, N, r.splits, stream);
 }
 
 template <typename OutT>
@@ -582,7 +710,13 @@ bool run_typed(const Route& r, int M, int N, int Kp, const void* dA, const void*
 }
 
 bool run(int ot, const Route& r, int M, int N, int Kp, const void* dA, const void* dB, const uint8_t* sA,
-         const uint8_t* sB, const kern::DstList& dl, int Ar, int Br, void* ws, cudaStream_t stream) {
+         const uint8_t* sB, const kern::DstList& dl, int Ar, int Br, void* ws, cudaStream_t stream,
+         const FusedLaunch* fused = nullptr) {
+    if (fused)
+        return a_mode(Kp, dA, Ar) == kern::A_TMA
+                   ? run_route<kern::FusedOut, kern::A_TMA>(r, M, N, Kp, dA, dB, sA, sB, dl, Ar, Br, ws, stream, fused)
+                   : run_route<kern::FusedOut, kern::A_CPASYNC>(r, M, N, Kp, dA, dB, sA, sB, dl, Ar, Br, ws, stream,
+                                                                fused);
     switch (ot) {
         case MXFP6_OUT_F32:
             return run_typed<float>(r, M, N, Kp, dA, dB, sA, sB, dl, Ar, Br, ws, stream);
@@ -684,15 +818,28 @@ void* repad_scratch_alloc(size_t bytes, cudaStream_t stream) {
     return p;
 }
 
+void run_validated(int ot, int M, int N, int Kp, const void* dA, const void* dB, const uint8_t* sA,
+                   const uint8_t* sB, const kern::DstList& dl, int Ar, int Br, void* ws, size_t ws_bytes,
+                   cudaStream_t stream, const FusedLaunch* fused = nullptr);
+
 void gemm_entry(int ot, int M, int N, int Kp, const void* dA, const void* dB, const uint8_t* sA,
                 const uint8_t* sB, const kern::DstList& dl, int Ar, int Br, void* ws, size_t ws_bytes,
                 cudaStream_t stream) {
     t_last_error = MXFP6_OK;
     if (!validate(ot, M, N, Kp, dA, dB, sA, sB, dl.p[0], Ar, Br)) return;
+    run_validated(ot, M, N, Kp, dA, dB, sA, sB, dl, Ar, Br, ws, ws_bytes, stream);
+}
+
+// The routed call on checked arguments: the workspace decides between the route and its unsplit form,
+// and a compact A is re-padded where there is room.
+void run_validated(int ot, int M, int N, int Kp, const void* dA, const void* dB, const uint8_t* sA,
+                   const uint8_t* sB, const kern::DstList& dl, int Ar, int Br, void* ws, size_t ws_bytes,
+                   cudaStream_t stream, const FusedLaunch* fused) {
     Route r = route_for_out(ot, M, N, Kp);
     const int sms = sm_count();
+    const int Nw = fused ? partials_pitch(N) : N;  // columns of the split-K partials
     if (r.splits > 1 || r.stream_k) {
-        const size_t need = route_ws_bytes(r, M, N, sms);
+        const size_t need = route_ws_bytes(r, M, Nw, sms);
         // the stream-K hand-off area takes 256-bit stores: a 256-byte aligned workspace
         if (!ws || ws_bytes < need || !aligned(ws, r.stream_k ? 256 : 16)) {
             // Same contract as the reference (src/dispatch.hpp:76-87): correct, only slower.
@@ -719,7 +866,7 @@ void gemm_entry(int ot, int M, int N, int Kp, const void* dA, const void* dB, co
     // large shapes).
     void* scratch = nullptr;
     if (a_mode(Kp, dA, Ar) == kern::A_CPASYNC) {
-        const size_t off = padded_a_offset(route_ws_bytes(r, M, N, sms));
+        const size_t off = padded_a_offset(route_ws_bytes(r, M, Nw, sms));
         const int prb = Kp / 4 * 3;
         uint8_t* pa = nullptr;
         if (ws && aligned(ws, 256) && ws_bytes >= off + padded_a_bytes(M, Kp))
@@ -739,9 +886,22 @@ void gemm_entry(int ot, int M, int N, int Kp, const void* dA, const void* dB, co
             Ar = prb;
         }
     }
-    run(ot, r, M, N, Kp, dA, dB, sA, sB, dl, Ar, Br, ws, stream);
+    run(ot, r, M, N, Kp, dA, dB, sA, sB, dl, Ar, Br, ws, stream, fused);
     if (scratch && cudaFreeAsync(scratch, stream) != cudaSuccess && t_last_error == MXFP6_OK)
         set_error(MXFP6_ERR_CUDA, "returning the A re-pad scratch failed: %s", cudaGetErrorString(cudaGetLastError()));
+}
+
+// Shape and operands of a fused call. Returns false when there is nothing to launch (an error is
+// recorded, or M == 0).
+bool validate_fused(int M, int N, int Kp, const void* dA, const void* dB, const void* sA, const void* sB,
+                    const void* dD, int Ar, int Br) {
+    if (M < 0 || N <= 0 || Kp <= 0 || Kp % K_TILE || N > (1 << 30)) {
+        set_error(MXFP6_ERR_INVALID_SHAPE,
+                  "unsupported fused shape %dx%dx%d: M >= 0, N > 0 and Kp a positive multiple of %d (pad with kpad())",
+                  M, N, Kp, K_TILE);
+        return false;
+    }
+    return M > 0 && validate_operands(Kp, dA, dB, sA, sB, dD, Ar, Br);
 }
 
 // ---- split-K scratch owned by the library (mxfp6_gemm_static_workspace) --------------------------------
@@ -1040,6 +1200,86 @@ void mxfp6_gemm_gather(int ot, int M, int N, int Kp, const void* dA, const void*
     dl.ldd = ldd;
     gemm_entry(ot, M, N, Kp, dA, dBsh, dsA, dsB, dl, A_row_bytes, B_row_bytes, ws, ws_bytes,
                static_cast<cudaStream_t>(stream));
+}
+
+int mxfp6_gemm_fused(int ot, int M, int N, int Kp, const void* dA, const void* dBsh, const uint8_t* dsA,
+                     const uint8_t* dsB, void* dD, long long ldd, int A_row_bytes, int B_row_bytes,
+                     const mxfp6_epilogue* epilogue, void* ws, size_t ws_bytes, void* stream) {
+    t_last_error = MXFP6_OK;
+    if (!valid_type(ot)) {
+        set_error(MXFP6_ERR_INVALID_OUT_TYPE, "invalid output type %d", ot);
+        return t_last_error;
+    }
+    FusedLaunch f;
+    if (!validate_fused(M, N, Kp, dA, dBsh, dsA, dsB, dD, A_row_bytes, B_row_bytes) ||
+        !validate_epilogue(epilogue, M, N, f.epi))
+        return t_last_error;
+    if (ldd < N) {
+        set_error(MXFP6_ERR_INVALID_STRIDE, "fused: output pitch %lld is below N = %d", ldd, N);
+        return t_last_error;
+    }
+    const int esize = type_bytes(ot);
+    if (!aligned(dD, esize)) {
+        set_error(MXFP6_ERR_MISALIGNED, "fused: D is not aligned to its element");
+        return t_last_error;
+    }
+    f.n_rows = N;
+    f.epi.out = dD;
+    f.epi.ldd = ldd;
+    f.epi.out_type = ot;
+    f.epi.out_vec = aligned(dD, 16) && (M == 1 || ldd * esize % 16 == 0);
+    run_validated(ot, M, N, Kp, dA, dBsh, dsA, dsB, kern::DstList{}, A_row_bytes, B_row_bytes, ws, ws_bytes,
+                  static_cast<cudaStream_t>(stream), &f);
+    return t_last_error;
+}
+
+int mxfp6_gemm_fused_quant(int M, int N, int Kp, const void* dA, const void* dBsh, const uint8_t* dsA,
+                           const uint8_t* dsB, uint8_t* d_packed, int packed_row_bytes, uint8_t* d_scales,
+                           int A_row_bytes, int B_row_bytes, const mxfp6_epilogue* epilogue, void* ws,
+                           size_t ws_bytes, void* stream) {
+    t_last_error = MXFP6_OK;
+    FusedLaunch f;
+    if (!validate_fused(M, N, Kp, dA, dBsh, dsA, dsB, d_packed, A_row_bytes, B_row_bytes) ||
+        !validate_epilogue(epilogue, M, N, f.epi))
+        return t_last_error;
+    if (N % K_TILE) {
+        set_error(MXFP6_ERR_INVALID_SHAPE, "fused: MXFP6 output needs N a multiple of %d, got %d", K_TILE, N);
+        return t_last_error;
+    }
+    if (!d_scales) {
+        set_error(MXFP6_ERR_NULL_POINTER, "fused: MXFP6 output without a scale buffer");
+        return t_last_error;
+    }
+    if (packed_row_bytes < N / 4 * 3 || packed_row_bytes % 32) {
+        set_error(MXFP6_ERR_INVALID_STRIDE,
+                  "fused: packed row stride %d bytes: must hold N = %d codes (%d bytes) and be a multiple of 32",
+                  packed_row_bytes, N, N / 4 * 3);
+        return t_last_error;
+    }
+    if (!aligned(d_packed, 32) || !aligned(d_scales, 16)) {
+        set_error(MXFP6_ERR_MISALIGNED, "fused: packed output needs 32-byte, its scales 16-byte alignment");
+        return t_last_error;
+    }
+    f.n_rows = N;
+    f.epi.out = d_packed;
+    f.epi.ldd = packed_row_bytes;
+    f.epi.scales = d_scales;
+    f.epi.out_type = kern::T_MXFP6;
+    f.epi.k_atoms = N / K_TILE;
+    run_validated(MXFP6_OUT_F16, M, N, Kp, dA, dBsh, dsA, dsB, kern::DstList{}, A_row_bytes, B_row_bytes, ws, ws_bytes,
+                  static_cast<cudaStream_t>(stream), &f);
+    return t_last_error;
+}
+
+size_t mxfp6_gemm_fused_workspace_size(int M, int N, int Kp, int A_row_bytes) {
+    if (M <= 0 || N <= 0 || Kp <= 0 || Kp % K_TILE) return 0;
+    size_t need = 0;
+    for (int ot : {MXFP6_OUT_F16, MXFP6_OUT_F32}) {
+        const size_t b = route_ws_bytes(route_for_out(ot, M, N, Kp), M, partials_pitch(N), sm_count());
+        if (b > need) need = b;
+    }
+    const bool tma_stride = A_row_bytes % 32 == 0 && (long long)A_row_bytes >= (long long)Kp * 3 / 4;
+    return tma_stride ? need : padded_a_offset(need) + padded_a_bytes(M, Kp);
 }
 
 int mxfp6_ipc_export(const void* dptr, void* handle_out, size_t* offset_out) {

@@ -33,6 +33,7 @@
 #include <type_traits>
 
 #include "compact_a.cuh"
+#include "epilogue.cuh"
 #include "sm100_ptx.cuh"
 
 namespace mxfp6 {
@@ -114,6 +115,16 @@ struct Params {
     // by band (partial band_L + j).
     int band_L, band_a, band_n;
 };
+
+// Output type tag of the launches with a fused epilogue (epilogue.cuh), whose parameters carry it;
+// D, its element type and its pitch are then in `epi`, and `dst` is unused. M and N may have any
+// positive value there: the tensor loads read zeros past the operands' last rows.
+struct FusedOut {};
+struct FusedParams : Params {
+    Epi epi;
+};
+template <typename OutT>
+using ParamsFor = std::conditional_t<std::is_same<OutT, FusedOut>::value, FusedParams, Params>;
 
 struct TileCoord {
     int mb, nb, split, kb_begin, kb_count;
@@ -236,13 +247,13 @@ __device__ __forceinline__ void store_rows_regrouped(const DstList& dl, uint8_t*
     __syncwarp();  // the staging area is rewritten by the next group
 }
 
-// OutT: float / __half / __nv_bfloat16. PARTIAL: write FP32 partial sums to p.ws instead of D.
+// OutT: float / __half / __nv_bfloat16, or FusedOut. PARTIAL: write FP32 partial sums to p.ws instead of D.
 // AMODE (compact_a.cuh): A_TMA loads A with the 16U6 tensor load; A_CPASYNC adds four
 // loader warps that copy the A image from p.a_ptr (tmA unused).
 template <int BN, typename OutT, bool PARTIAL, int AMODE = A_TMA>
 __global__ void __launch_bounds__(threads_for(AMODE), 1)
     gemm_mxfp6_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                     const Params p) {
+                     const ParamsFor<OutT> p) {
     using C = Config<BN, AMODE>;
     constexpr bool COMPACT = AMODE != A_TMA;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -448,6 +459,8 @@ __global__ void __launch_bounds__(threads_for(AMODE), 1)
                     if constexpr (PARTIAL) {
                         float* dst = p.ws + ((size_t)tc.split * p.M + row) * p.N + col0 + c;
                         store_words<32>(dst, r, p.out_align32 != 0);
+                    } else if constexpr (std::is_same<OutT, FusedOut>::value) {
+                        epi_chunk(p.epi, row, col0 + c, p.N - col0 - c, r);
                     } else {
                         uint32_t w[ChunkWords<OutT>::N];
                         convert_chunk<OutT>(r, w);
@@ -531,6 +544,61 @@ __global__ void __launch_bounds__(256) reduce_partials(const float* __restrict__
             const uint2 o = make_uint2(*reinterpret_cast<uint32_t*>(&lo), *reinterpret_cast<uint32_t*>(&hi));
             for (int d = 0; d < dl.n; d++)
                 *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(dl.p[d]) + off) = o;
+        }
+    }
+}
+
+// Split-K second stage of a fused launch: the same sum in the same order, then the fused epilogue.
+// The partials have a pitch of Np columns (N rounded up to 32). A thread takes four columns; the
+// eight threads of a 32-column block are consecutive lanes of one warp (blocks never straddle: Np is
+// a multiple of 32), so MXFP6 output takes the block's maximum over three shuffles.
+__global__ void __launch_bounds__(256) reduce_partials_fused(const float* __restrict__ ws, const Epi e, int M, int N,
+                                                             int Np, int S) {
+    sm100::griddep_launch_dependents();
+    sm100::griddep_wait();  // the partials of the GEMM before it
+    const long long total = (long long)M * Np, n4 = total / 4;
+    const long long step = (long long)gridDim.x * blockDim.x;
+    // whole warps stay in the loop together: n4 is a multiple of 8, so a block's lanes agree
+    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i - (threadIdx.x & 31) < n4; i += step) {
+        const bool live = i < n4;
+        const int row = live ? (int)(4 * i / Np) : 0;
+        const int col = live ? (int)(4 * i - (long long)row * Np) : 0;
+        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (live) {
+            const float4 first = reinterpret_cast<const float4*>(ws)[i];
+            v[0] = first.x;
+            v[1] = first.y;
+            v[2] = first.z;
+            v[3] = first.w;
+            for (int s = 1; s < S; s++) {
+                const float4 q = reinterpret_cast<const float4*>(ws + (size_t)s * total)[i];
+                v[0] += q.x;
+                v[1] += q.y;
+                v[2] += q.z;
+                v[3] += q.w;
+            }
+        }
+        const int valid = live ? N - col : 0;
+        epi_apply4(e, row, col, valid, v);
+        if (e.out_type != T_MXFP6) {
+            store_elems4(e, row, col, valid, v);
+            continue;
+        }
+        float m = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+#pragma unroll
+        for (int d = 1; d < 8; d *= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+        const uint32_t code = scale_code(m);
+        const float inv = e8m0_reciprocal(code);
+        const uint32_t lo = to_e2m3x2(v[1] * inv, v[0] * inv), hi = to_e2m3x2(v[3] * inv, v[2] * inv);
+        const uint32_t g = (lo & 0x3Fu) | ((lo >> 2) & 0xFC0u) | ((hi & 0x3Fu) << 12) | ((hi << 10) & 0xFC0000u);
+        // four lanes' 24-bit groups -> three words, written by the quad's first three lanes
+        const uint32_t next = __shfl_down_sync(0xffffffffu, g, 1);
+        const int q = threadIdx.x & 3;
+        const uint32_t w = q == 0 ? g | (next << 24) : q == 1 ? (g >> 8) | (next << 16) : (g >> 16) | (next << 8);
+        if (live) {
+            uint8_t* d = static_cast<uint8_t*>(e.out) + (size_t)row * (size_t)e.ldd + (size_t)((col & ~15) / 4 * 3);
+            if (q < 3) reinterpret_cast<uint32_t*>(d)[q] = w;
+            if ((threadIdx.x & 7) == 0) e.scales[scale_atom_offset(row, col / 32, e.k_atoms)] = (uint8_t)code;
         }
     }
 }

@@ -204,7 +204,7 @@ template <typename OutT, bool PARTIAL, int AMODE = A_TMA, int EPI = EPI_ALL>
 __global__ void __launch_bounds__(threads_for(AMODE), 1)
     gemm_mxfp6_sm100_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                           const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB,
-                          const Params p) {
+                          const ParamsFor<OutT> p) {
     using C = PairConfig<AMODE>;
     constexpr bool COMPACT = AMODE != A_TMA;
     static_assert(C::SUB == 1, "one 128-deep slab per stage");
@@ -605,6 +605,8 @@ __global__ void __launch_bounds__(threads_for(AMODE), 1)
                 } else if (row < p.M && col < p.N) {
                     if constexpr (PARTIAL) {
                         store_words<32>(p.ws + ((size_t)tc.split * p.M + row) * p.N + col, r, p.out_align32 != 0);
+                    } else if constexpr (std::is_same<OutT, FusedOut>::value) {
+                        epi_chunk(p.epi, row, col, p.N - col, r);
                     } else {
                         uint32_t w[ChunkWords<OutT>::N];
                         convert_chunk<OutT>(r, w);

@@ -1,0 +1,83 @@
+#pragma once
+// Device pieces of MXFP6 quantisation shared by the quantisers (quantize.cu) and the kernels that
+// write MXFP6 themselves (epilogue.cuh, moe.cu). Per 32 values: scale = smallest power of two
+// >= max|x| / 7.5 (E8M0 code, 127 for a block of zeros, NaN ignored by the max), codes = nearest
+// E2M3 of x / scale, packed four codes per three bytes, least significant bits first.
+#include <cstdint>
+
+namespace mxfp6 {
+
+// E8M0 code of the smallest power of two >= v (v > 0, finite or +Inf): from the float bits,
+// the same result as frexp-based rounding up (a power of two maps to itself).
+__device__ __forceinline__ uint32_t ceil_pow2_code(float v) {
+    const uint32_t b = __float_as_uint(v);
+    if (b >= 0x7F800000u) return 127;  // +Inf: the reference's frexp reports exponent 0
+    int e;                              // v = m * 2^e with m in [1, 2)
+    uint32_t man;
+    if (b >= 0x00800000u) {
+        e = (int)(b >> 23) - 127;
+        man = b & 0x7FFFFFu;
+    } else {  // subnormal: normalise the mantissa
+        const int lz = __clz(b) - 8;    // leading zeros within the 24-bit significand field
+        e = -126 - lz;
+        man = (b << lz) & 0x7FFFFFu;
+    }
+    const int code = e + (man != 0 ? 1 : 0) + 127;
+    return (uint32_t)(code < 0 ? 0 : (code > 254 ? 254 : code));
+}
+
+// E8M0 code of the reference's block scale for block max m >= 0: the smallest power of two
+// >= RN(m / 7.5), 127 for m == 0. For P = 2^e >= 2^-125, RN(m / 7.5) <= P exactly when
+// m <= 7.5 * P (the rounding boundary P + ulp(P)/2 lies below the next float above 7.5 * P), so
+// with m = 1.f * 2^E the code is E - 2, plus 1 when the mantissa exceeds 1.875, plus the bias.
+// Subnormal quotients, an infinite max and m == 0 take the division.
+__device__ __forceinline__ uint32_t scale_code(float m) {
+    const uint32_t mb = __float_as_uint(m);
+    const int e = (int)(mb >> 23) - 129 + ((mb & 0x7FFFFFu) > 0x700000u ? 1 : 0);
+    if (mb < 0x7F800000u && (mb >> 23) != 0u && e >= -125) return (uint32_t)(e + 127);
+    return m == 0.0f ? 127u : ceil_pow2_code(__fdiv_rn(m, 7.5f));
+}
+
+// Nearest E2M3 codes of two values (round to nearest even, saturating at 7.5) with the
+// hardware conversion cvt.rn.satfinite.e2m3x2.f32, which writes a's code to the upper byte and
+// b's to the lower one. Two inputs are first replaced so that the codes equal the reference's
+// conversion (include/mxfp6/types.hpp:26-72): NaN -> 4.0 (code 0x18, what the reference yields on
+// x86-64) and -0.0 -> +0.0 (code 0; other negatives that round to zero keep the sign, 0x20).
+// Returns code(b) | code(a) << 8.
+__device__ __forceinline__ uint32_t to_e2m3x2(float a, float b) {
+    a = a != a ? 4.0f : a + 0.0f;
+    b = b != b ? 4.0f : b + 0.0f;
+    uint16_t d;
+    asm("cvt.rn.satfinite.e2m3x2.f32 %0, %1, %2;" : "=h"(d) : "f"(a), "f"(b));
+    return d;
+}
+
+// 1 / 2^(code - 127) = 2^(127 - code), exact for every code the quantiser produces (0..254):
+// multiplying by it rounds exactly like dividing by the scale.
+__device__ __forceinline__ float e8m0_reciprocal(uint32_t code) {
+    const int e = 254 - (int)code;  // biased exponent of 2^(127 - code)
+    return e > 0 ? __int_as_float(e << 23) : __int_as_float(0x00400000 >> (-e));
+}
+
+// 16 values times `inv`, as 16 codes in three words (bits 6k of 96).
+__device__ __forceinline__ void quantize16(const float* v, float inv, uint32_t& w0, uint32_t& w1, uint32_t& w2) {
+    uint32_t c[16];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const uint32_t q = to_e2m3x2(v[2 * i + 1] * inv, v[2 * i] * inv);
+        c[2 * i] = q & 0x3Fu;
+        c[2 * i + 1] = (q >> 8) & 0x3Fu;
+    }
+    w0 = c[0] | (c[1] << 6) | (c[2] << 12) | (c[3] << 18) | (c[4] << 24) | (c[5] << 30);
+    w1 = (c[5] >> 2) | (c[6] << 4) | (c[7] << 10) | (c[8] << 16) | (c[9] << 22) | (c[10] << 28);
+    w2 = (c[10] >> 4) | (c[11] << 2) | (c[12] << 8) | (c[13] << 14) | (c[14] << 20) | (c[15] << 26);
+}
+
+// Byte offset of the scale of (row, 32-column block j) in the GEMM's atoms of 128 rows x 4 blocks;
+// k_atoms = columns / 128.
+__device__ __forceinline__ size_t scale_atom_offset(int row, int j, int k_atoms) {
+    const size_t atom = (size_t)(row / 128) * (size_t)k_atoms + (size_t)(j / 4);
+    return atom * 512 + (size_t)((row % 32) * 16 + ((row % 128) / 32) * 4 + (j % 4));
+}
+
+}  // namespace mxfp6

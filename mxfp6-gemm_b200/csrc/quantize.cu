@@ -17,6 +17,8 @@
 #include <cstdio>
 
 #include "mxfp6_gemm.h"
+#include "epilogue.cuh"
+#include "quant.cuh"
 #include "sm100_ptx.cuh"
 
 namespace mxfp6 {
@@ -24,57 +26,20 @@ void note_launch();  // launch counter (gemm.cu)
 
 namespace {
 
-// E8M0 code of the smallest power of two >= v (v > 0, finite or +Inf): from the float bits,
-// the same result as frexp-based rounding up (a power of two maps to itself).
-__device__ __forceinline__ uint32_t ceil_pow2_code(float v) {
-    const uint32_t b = __float_as_uint(v);
-    if (b >= 0x7F800000u) return 127;  // +Inf: the reference's frexp reports exponent 0
-    int e;                              // v = m * 2^e with m in [1, 2)
-    uint32_t man;
-    if (b >= 0x00800000u) {
-        e = (int)(b >> 23) - 127;
-        man = b & 0x7FFFFFu;
-    } else {  // subnormal: normalise the mantissa
-        const int lz = __clz(b) - 8;    // leading zeros within the 24-bit significand field
-        e = -126 - lz;
-        man = (b << lz) & 0x7FFFFFu;
-    }
-    const int code = e + (man != 0 ? 1 : 0) + 127;
-    return (uint32_t)(code < 0 ? 0 : (code > 254 ? 254 : code));
-}
-
-// E8M0 code of the reference's block scale for block max m >= 0: the smallest power of two
-// >= RN(m / 7.5), 127 for m == 0. For P = 2^e >= 2^-125, RN(m / 7.5) <= P exactly when
-// m <= 7.5 * P (the rounding boundary P + ulp(P)/2 lies below the next float above 7.5 * P), so
-// with m = 1.f * 2^E the code is E - 2, plus 1 when the mantissa exceeds 1.875, plus the bias.
-// Subnormal quotients, an infinite max and m == 0 take the division.
-__device__ __forceinline__ uint32_t scale_code(float m) {
-    const uint32_t mb = __float_as_uint(m);
-    const int e = (int)(mb >> 23) - 129 + ((mb & 0x7FFFFFu) > 0x700000u ? 1 : 0);
-    if (mb < 0x7F800000u && (mb >> 23) != 0u && e >= -125) return (uint32_t)(e + 127);
-    return m == 0.0f ? 127u : ceil_pow2_code(__fdiv_rn(m, 7.5f));
-}
-
-// Nearest E2M3 codes of two values (round to nearest even, saturating at 7.5) with the
-// hardware conversion cvt.rn.satfinite.e2m3x2.f32, which writes a's code to the upper byte and
-// b's to the lower one. Two inputs are first replaced so that the codes equal the reference's
-// conversion (include/mxfp6/types.hpp:26-72): NaN -> 4.0 (code 0x18, what the reference yields on
-// x86-64) and -0.0 -> +0.0 (code 0; other negatives that round to zero keep the sign, 0x20).
-// Returns code(b) | code(a) << 8.
-__device__ __forceinline__ uint32_t to_e2m3x2(float a, float b) {
-    a = a != a ? 4.0f : a + 0.0f;
-    b = b != b ? 4.0f : b + 0.0f;
-    uint16_t d;
-    asm("cvt.rn.satfinite.e2m3x2.f32 %0, %1, %2;" : "=h"(d) : "f"(a), "f"(b));
-    return d;
-}
-
-// 1 / 2^(code - 127) = 2^(127 - code), exact for every code the quantiser produces (0..254):
-// multiplying by it rounds exactly like dividing by the scale.
-__device__ __forceinline__ float e8m0_reciprocal(uint32_t code) {
-    const int e = 254 - (int)code;  // biased exponent of 2^(127 - code)
-    return e > 0 ? __int_as_float(e << 23) : __int_as_float(0x00400000 >> (-e));
-}
+template <typename T>
+struct TypeOf;
+template <>
+struct TypeOf<float> {
+    static constexpr int value = kern::T_F32;
+};
+template <>
+struct TypeOf<__half> {
+    static constexpr int value = kern::T_F16;
+};
+template <>
+struct TypeOf<__nv_bfloat16> {
+    static constexpr int value = kern::T_BF16;
+};
 
 // One warp quantises a 512-element chunk of a row: lane l owns the 16 consecutive values
 // [16 l, 16 l + 16), so each 32-value block spans the lane pair (2b, 2b + 1) (one shuffle for its
@@ -111,19 +76,8 @@ __global__ void __launch_bounds__(256) quantize_kernel(const float* __restrict__
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
     const uint32_t code = scale_code(m);
     const float inv = e8m0_reciprocal(code);
-    uint32_t q[8];  // q[i] = code(v[2i]) | code(v[2i + 1]) << 8
-#pragma unroll
-    for (int i = 0; i < 8; i++) q[i] = to_e2m3x2(v[2 * i + 1] * inv, v[2 * i] * inv);
-    // codes c0..c15 (6 bits each) -> bits 6k of three words
-    uint32_t c[16];
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        c[2 * i] = q[i] & 0x3Fu;
-        c[2 * i + 1] = (q[i] >> 8) & 0x3Fu;
-    }
-    const uint32_t w0 = c[0] | (c[1] << 6) | (c[2] << 12) | (c[3] << 18) | (c[4] << 24) | (c[5] << 30);
-    const uint32_t w1 = (c[5] >> 2) | (c[6] << 4) | (c[7] << 10) | (c[8] << 16) | (c[9] << 22) | (c[10] << 28);
-    const uint32_t w2 = (c[10] >> 4) | (c[11] << 2) | (c[12] << 8) | (c[13] << 14) | (c[14] << 20) | (c[15] << 26);
+    uint32_t w0, w1, w2;
+    quantize16(v, inv, w0, w1, w2);
     if (live) {
         uint32_t* dst = reinterpret_cast<uint32_t*>(packed + (size_t)row * out_row_bytes + (size_t)col / 4 * 3);
         dst[0] = w0;
@@ -138,6 +92,49 @@ __global__ void __launch_bounds__(256) quantize_kernel(const float* __restrict__
             } else {
                 off = (size_t)row * scale_cols + j;
             }
+            scales[off] = (uint8_t)code;
+        }
+    }
+}
+
+// The quantiser for any input type and row stride, padding in the same pass: the lane layout of
+// quantize_kernel, with rows as a grid-stride loop and the tail [cols, padded_cols) written as zero
+// codes with the finite scale 127. HBM bound: a BF16 element reads 2 bytes and writes 0.78.
+// VEC: 16-byte aligned rows (ld and base), so a lane's 16 values are two (four for FP32) wide loads.
+template <typename In, bool VEC>
+__global__ void __launch_bounds__(256) quantize_rows_kernel(const In* __restrict__ in, int rows, int cols, long long ld,
+                                                            int padded_cols, uint8_t* __restrict__ packed,
+                                                            uint8_t* __restrict__ scales, int tiled) {
+    sm100::griddep_launch_dependents();
+    sm100::griddep_wait();  // launched with programmatic stream serialization
+    const int lane = threadIdx.x & 31;
+    const int chunk = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    if ((long long)chunk * 512 >= padded_cols) return;
+    const int col = chunk * 512 + 16 * lane;
+    const bool live = col < cols;  // cols % 32 == 0: a lane's 16 values are all in or all out
+    const bool kept = col < padded_cols;
+    const size_t out_row_bytes = (size_t)(padded_cols / 4 * 3);
+    for (int row = blockIdx.y; row < rows; row += gridDim.y) {
+        float v[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) v[i] = 0.0f;
+        if (live) kern::load_elems<16>(in, TypeOf<In>::value, (size_t)row * (size_t)ld + (size_t)col, 16, VEC, v);
+        float m = 0.0f;  // fmaxf returns the other operand for a NaN: NaN never wins the max
+#pragma unroll
+        for (int i = 0; i < 16; i++) m = fmaxf(m, fabsf(v[i]));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        const uint32_t code = scale_code(m);
+        uint32_t w0, w1, w2;
+        quantize16(v, e8m0_reciprocal(code), w0, w1, w2);
+        if (!kept) continue;
+        uint32_t* dst = reinterpret_cast<uint32_t*>(packed + (size_t)row * out_row_bytes + (size_t)(col / 4 * 3));
+        dst[0] = w0;
+        dst[1] = w1;
+        dst[2] = w2;
+        if ((lane & 1) == 0) {
+            const int j = col / 32;
+            const size_t off = tiled ? scale_atom_offset(row, j, padded_cols / 128)
+                                     : (size_t)row * (size_t)(padded_cols / 32) + (size_t)j;
             scales[off] = (uint8_t)code;
         }
     }
@@ -194,6 +191,25 @@ __global__ void __launch_bounds__(256) repad_kernel(const uint8_t* __restrict__ 
 }
 
 }  // namespace
+
+template <typename In>
+cudaError_t launch_quantize_rows(const In* in, int rows, int cols, long long ld, int padded_cols, uint8_t* packed,
+                                 uint8_t* scales, int tiled, cudaStream_t stream) {
+    const bool vec = (reinterpret_cast<uintptr_t>(in) & 15) == 0 && (rows == 1 || ld * (long long)sizeof(In) % 16 == 0);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((padded_cols + 4095) / 4096), (unsigned)(rows < 65535 ? rows : 65535), 1);
+    cfg.blockDim = dim3(256, 1, 1);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return vec ? cudaLaunchKernelEx(&cfg, quantize_rows_kernel<In, true>, in, rows, cols, ld, padded_cols, packed, scales,
+                                    tiled)
+               : cudaLaunchKernelEx(&cfg, quantize_rows_kernel<In, false>, in, rows, cols, ld, padded_cols, packed,
+                                    scales, tiled);
+}
 
 // Launch the re-pad copy with the widest unit the pointers and strides allow (used by
 // mxfp6_repad_rows_device and by gemm() for compact A with a large enough workspace).
@@ -255,6 +271,53 @@ extern "C" int mxfp6_quantize_device_padded(const float* d_mat, int rows, int co
     }
     if (e != cudaSuccess) {
         std::fprintf(stderr, "[mxfp6] quantize_device launch failed: %s\n", cudaGetErrorString(e));
+        return MXFP6_ERR_CUDA;
+    }
+    note_launch();
+    return MXFP6_OK;
+}
+
+extern "C" int mxfp6_quantize_device_typed(const void* d_mat, int in_type, int rows, int cols, long long ld,
+                                           int padded_cols, uint8_t* d_packed, uint8_t* d_scales, int scale_layout,
+                                           void* stream) {
+    using namespace mxfp6;
+    if (in_type < MXFP6_OUT_F32 || in_type > MXFP6_OUT_BF16) {
+        std::fprintf(stderr, "[mxfp6] quantize_device_typed: invalid input type %d\n", in_type);
+        return MXFP6_ERR_INVALID_OUT_TYPE;
+    }
+    if (rows < 0 || cols <= 0 || cols % 32 || padded_cols < cols || padded_cols % 32 ||
+        (scale_layout != 0 && scale_layout != 1) || (scale_layout == 1 && padded_cols % 128)) {
+        std::fprintf(stderr, "[mxfp6] quantize_device_typed: invalid arguments (%d x %d padded to %d, layout %d)\n", rows,
+                     cols, padded_cols, scale_layout);
+        return MXFP6_ERR_INVALID_SHAPE;
+    }
+    if (rows == 0) return MXFP6_OK;
+    if (!d_mat || !d_packed || !d_scales) {
+        std::fprintf(stderr, "[mxfp6] quantize_device_typed: null device pointer\n");
+        return MXFP6_ERR_NULL_POINTER;
+    }
+    if (ld < cols) {
+        std::fprintf(stderr, "[mxfp6] quantize_device_typed: row stride %lld is below cols = %d\n", ld, cols);
+        return MXFP6_ERR_INVALID_STRIDE;
+    }
+    const uintptr_t esize = in_type == MXFP6_OUT_F32 ? 4 : 2;
+    if ((reinterpret_cast<uintptr_t>(d_mat) & (esize - 1)) || (reinterpret_cast<uintptr_t>(d_packed) & 3)) {
+        std::fprintf(stderr, "[mxfp6] quantize_device_typed: input must be aligned to its element, output to 4 bytes\n");
+        return MXFP6_ERR_MISALIGNED;
+    }
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const cudaError_t e =
+        in_type == MXFP6_OUT_F32
+            ? launch_quantize_rows(static_cast<const float*>(d_mat), rows, cols, ld, padded_cols, d_packed, d_scales,
+                                   scale_layout, st)
+        : in_type == MXFP6_OUT_F16
+            ? launch_quantize_rows(static_cast<const __half*>(d_mat), rows, cols, ld, padded_cols, d_packed, d_scales,
+                                   scale_layout, st)
+            : launch_quantize_rows(static_cast<const __nv_bfloat16*>(d_mat), rows, cols, ld, padded_cols, d_packed,
+                                   d_scales, scale_layout, st);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        std::fprintf(stderr, "[mxfp6] quantize_device_typed launch failed: %s\n", cudaGetErrorString(e));
         return MXFP6_ERR_CUDA;
     }
     note_launch();

@@ -66,6 +66,20 @@ _gather = _fn("mxfp6_gemm_gather", None,
               [C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                C.POINTER(C.c_void_p), C.c_int, C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_size_t,
                C.c_void_p])
+
+
+class _EpilogueStruct(C.Structure):  # mxfp6_epilogue
+    _fields_ = [("bias", C.c_void_p), ("aux", C.c_void_p), ("ld_aux", C.c_longlong), ("bias_type", C.c_int),
+                ("activation", C.c_int), ("aux_op", C.c_int), ("aux_type", C.c_int)]
+
+
+_gemm_fused = _fn("mxfp6_gemm_fused", C.c_int,
+                  [C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                   C.c_longlong, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p])
+_gemm_fused_q = _fn("mxfp6_gemm_fused_quant", C.c_int,
+                    [C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int,
+                     C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p])
+_ws_fused = _fn("mxfp6_gemm_fused_workspace_size", C.c_size_t, [C.c_int, C.c_int, C.c_int, C.c_int])
 _ipc_export = _fn("mxfp6_ipc_export", C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(C.c_size_t)])
 _ipc_import = _fn("mxfp6_ipc_import", C.c_int, [C.c_void_p, C.c_size_t, C.POINTER(C.c_void_p),
                                                C.POINTER(C.c_void_p)])
@@ -88,6 +102,9 @@ _quantize_dev = _fn("mxfp6_quantize_device", C.c_int,
                     [C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p])
 _quantize_dev_p = _fn("mxfp6_quantize_device_padded", C.c_int,
                       [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p])
+_quantize_dev_t = _fn("mxfp6_quantize_device_typed", C.c_int,
+                      [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_longlong, C.c_int, C.c_void_p, C.c_void_p, C.c_int,
+                       C.c_void_p])
 _imp_B_dev = _fn("mxfp6_import_ref_B_device", C.c_int,
                  [C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_int, C.c_void_p])
 _imp_sc_dev = _fn("mxfp6_import_ref_scales_device", C.c_int,
@@ -111,6 +128,22 @@ class OutType(enum.IntEnum):
     F32 = 0
     F16 = 1
     BF16 = 2
+
+
+class Act(enum.IntEnum):
+    """Activation of a fused epilogue (enum mxfp6_activation)."""
+    NONE = 0
+    RELU = 1
+    GELU = 2
+    GELU_TANH = 3
+    SILU = 4
+
+
+class AuxOp(enum.IntEnum):
+    """How a fused epilogue's aux operand joins (enum mxfp6_aux_op)."""
+    NONE = 0
+    ADD = 1
+    MUL = 2
 
 
 K_TILE = _k_tile()
@@ -217,6 +250,47 @@ def gemm_gather(ot, M, N, Kp, dA, dBsh, dsA, dsB, dDs, ldd, col0, A_row_bytes, B
             A_row_bytes, B_row_bytes, _addr(ws), ws_bytes, s)
 
 
+class Epilogue:
+    """The epilogue of gemm_fused / gemm_fused_quant (struct mxfp6_epilogue): op(act(A·B + bias), aux).
+    bias: N elements of bias_type; aux: [M][ld_aux] of aux_type (ld_aux may be left out for a tensor,
+    whose row stride it then is). Build it once and pass it to any number of calls; it keeps the
+    operands it was given alive."""
+
+    def __init__(self, bias=None, bias_type=OutType.F32, act=Act.NONE, aux=None, aux_type=OutType.F32,
+                 aux_op=AuxOp.NONE, ld_aux=None):
+        if ld_aux is None:
+            if isinstance(aux, int):
+                raise ValueError("ld_aux is needed for an aux operand given as an address")
+            ld_aux = 0 if aux is None else aux.stride(0)
+        self.keep = (bias, aux)
+        self.struct = _EpilogueStruct(_addr(bias), _addr(aux), ld_aux, int(bias_type), int(act), int(aux_op),
+                                      int(aux_type))
+        self.ref = C.addressof(self.struct)
+
+
+def gemm_fused(ot, M, N, Kp, dA, dBsh, dsA, dsB, dD, A_row_bytes, B_row_bytes, epilogue=None, ws=None, ws_bytes=0,
+               stream=None, ldd=None) -> int:
+    """mxfp6_gemm_fused: D = op(act(A·B + bias), aux) for any M >= 0 and N > 0, rows of D ldd
+    elements apart (N by default). Asynchronous; returns an mxfp6_status."""
+    return _gemm_fused(int(ot), M, N, Kp, _addr(dA), _addr(dBsh), _addr(dsA), _addr(dsB), _addr(dD),
+                       N if ldd is None else ldd, A_row_bytes, B_row_bytes, epilogue.ref if epilogue else 0,
+                       _addr(ws), ws_bytes, _stream_arg(stream))
+
+
+def gemm_fused_quant(M, N, Kp, dA, dBsh, dsA, dsB, d_packed, d_scales, A_row_bytes, B_row_bytes, epilogue=None,
+                     ws=None, ws_bytes=0, stream=None, packed_row_bytes=None) -> int:
+    """mxfp6_gemm_fused_quant: the same, quantised to MXFP6 rows (3N/4 bytes apart by default) and
+    tiled scales: the A operand of a following GEMM. Returns an mxfp6_status."""
+    return _gemm_fused_q(M, N, Kp, _addr(dA), _addr(dBsh), _addr(dsA), _addr(dsB), _addr(d_packed),
+                         N * 3 // 4 if packed_row_bytes is None else packed_row_bytes, _addr(d_scales), A_row_bytes,
+                         B_row_bytes, epilogue.ref if epilogue else 0, _addr(ws), ws_bytes, _stream_arg(stream))
+
+
+def gemm_fused_workspace_size(M: int, N: int, Kp: int, a_row_bytes: int | None = None) -> int:
+    """Workspace bytes of gemm_fused / gemm_fused_quant for an A of row stride a_row_bytes (0.75*Kp)."""
+    return _ws_fused(M, N, Kp, Kp * 3 // 4 if a_row_bytes is None else a_row_bytes)
+
+
 def ipc_export(t) -> tuple[bytes, int]:
     """(64-byte CUDA IPC handle of the allocation holding t, t's offset in it)."""
     h = (C.c_uint8 * 64)()
@@ -297,6 +371,14 @@ def quantize_device_padded(d_mat, rows, cols, padded_cols, d_packed, d_scales, t
     s = 0 if stream is None else (stream.cuda_stream if hasattr(stream, "cuda_stream") else _addr(stream))
     return _quantize_dev_p(_addr(d_mat), rows, cols, padded_cols, _addr(d_packed), _addr(d_scales),
                            1 if tiled else 0, s)
+
+
+def quantize_device_typed(d_mat, in_type, rows, cols, ld, padded_cols, d_packed, d_scales, tiled=False,
+                          stream=None) -> int:
+    """mxfp6_quantize_device_typed: rows of F32 / F16 / BF16 values, ld elements apart, quantised to
+    rows of padded_cols codes (device pointers). Returns an mxfp6_status."""
+    return _quantize_dev_t(_addr(d_mat), int(in_type), rows, cols, ld, padded_cols, _addr(d_packed), _addr(d_scales),
+                           1 if tiled else 0, _stream_arg(stream))
 
 
 def repad_rows_device(d_src, rows, src_row_bytes, bytes_used, d_dst, dst_row_bytes, stream=None) -> int:

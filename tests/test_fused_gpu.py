@@ -1,0 +1,274 @@
+"""Fused-epilogue GEMM (mxfp6_gemm_fused, mxfp6_gemm_fused_quant) and the typed quantiser against FP64
+restatements of their formulas, over routes, odd sizes, strides, types and activations."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import mxfp6_b200 as lib
+from fused_ref import DTYPE, Operand, check_quantised, check_rounded, fused64
+from mxfp6_b200 import Act, AuxOp, OutType
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _cuda():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+
+
+def _workspace(A, N, poison=True):
+    n = lib.gemm_fused_workspace_size(A.rows, N, A.Kp, A.row_bytes)
+    return (torch.full((n,), 0x5A, dtype=torch.uint8, device="cuda") if n else None), n
+
+
+def _finish():
+    torch.cuda.synchronize()
+    assert lib.device_status() == 0
+
+
+def _randn(*shape, seed, std=1.0, dtype=torch.float32):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(*shape, generator=g, device="cuda") * std).to(dtype)
+
+
+def _fused(A, B, ot, act=Act.NONE, bias=None, bias_type=OutType.F32, aux=None, aux_type=OutType.F32, aux_op=AuxOp.NONE,
+           ldd=None, offset=0, ws=True, stream=None):
+    """Runs the call into a poisoned buffer with rows ldd apart, `offset` elements past an aligned base,
+    and checks that nothing outside D was written."""
+    M, N = A.rows, B.rows
+    ldd = ldd or N
+    buf = torch.full((offset + (M + 1) * ldd,), 1234.0, dtype=DTYPE[ot], device="cuda")
+    D = buf[offset:offset + M * ldd].view(M, ldd)
+    w, n = _workspace(A, N) if ws else (None, 0)
+    ep = lib.Epilogue(bias, bias_type, act, aux, aux_type, aux_op)
+    rc = lib.gemm_fused(ot, M, N, A.Kp, A.packed, B.packed, A.scales, B.scales, D, A.row_bytes, B.row_bytes, ep, w, n,
+                        ldd=ldd, stream=stream)
+    assert rc == lib.OK, lib.last_error_string()
+    _finish()
+    assert (buf[:offset] == 1234.0).all() and (D[:, N:] == 1234.0).all() and (buf[offset + M * ldd:] == 1234.0).all()
+    return D[:, :N]
+
+
+# Sizes that end inside tiles, chunks and scale atoms, on every tile and on split K; F32 rounds nothing.
+@pytest.mark.parametrize("M,N,K", [(1, 1, 128), (1, 4096, 4096), (3, 33, 160), (5, 1000, 2080), (127, 129, 512),
+                                   (129, 31, 96), (200, 264, 1024), (257, 513, 384), (1000, 2056, 768),
+                                   (1, 128, 8192), (300, 2500, 512), (2049, 2500, 256)])
+@pytest.mark.parametrize("ot", list(OutType))
+def test_sizes(M, N, K, ot):
+    A, B = Operand(M, K, 1.0, M + K), Operand(N, K, K ** -0.5, N + K)
+    bias = _randn(N, seed=1)
+    got = _fused(A, B, ot, Act.SILU, bias)
+    check_rounded(got, *fused64(A, B, Act.SILU, bias, None, AuxOp.NONE), ot, f"{M}x{N}x{K}")
+
+
+@pytest.mark.parametrize("act", list(Act))
+@pytest.mark.parametrize("aux_op", list(AuxOp))
+def test_activations_and_aux(act, aux_op):
+    M, N, K = 70, 200, 256
+    A, B = Operand(M, K, 2.0, 3), Operand(N, K, 0.1, 4)
+    for ot, bt, at in ((OutType.F32, OutType.BF16, OutType.F16), (OutType.F16, OutType.F32, OutType.BF16),
+                       (OutType.BF16, OutType.F16, OutType.F32)):
+        bias, aux = _randn(N, seed=5, dtype=DTYPE[bt]), _randn(M, N + 9, seed=6, dtype=DTYPE[at])[:, 4:N + 4]
+        got = _fused(A, B, ot, act, bias, bt, aux, at, aux_op)
+        check_rounded(got, *fused64(A, B, act, bias, aux, aux_op), ot, f"{act.name} {aux_op.name} {ot.name}")
+
+
+# Pitches and bases that allow wide accesses, 16-byte ones only by chance, or none.
+@pytest.mark.parametrize("ldd,offset", [(256, 0), (264, 8), (257, 0), (300, 1), (256, 3)])
+@pytest.mark.parametrize("ot", list(OutType))
+def test_output_strides(ldd, offset, ot):
+    A, B = Operand(140, 256, 1.0, 7), Operand(256, 256, 0.06, 8)
+    got = _fused(A, B, ot, ldd=ldd, offset=offset)
+    check_rounded(got, *fused64(A, B, Act.NONE, None, None, AuxOp.NONE), ot)
+
+
+def _route_of(ot, M, N, K):
+    return lib.route(ot, M, N, lib.kpad(K))
+
+
+# One shape for each schedule: whole tiles on the pair, split K, stream-K tail, banded split.
+@pytest.mark.parametrize("M,N,K,want", [(4096, 4700, 256, "pair"), (256, 250, 8192, "splits"),
+                                        (4090, 3570, 6144, "stream_k"), (1500, 2040, 24576, "banded")])
+def test_schedules(M, N, K, want):
+    r = _route_of(OutType.BF16, M, N, K)
+    assert (r["MT"] == 256 if want == "pair" else r["splits"] > 1 if want == "splits" else r[want]), r
+    A, B = Operand(M, K, 1.0, 9), Operand(N, K, K ** -0.5, 10)
+    bias, aux = _randn(N, seed=11), _randn(M, N, seed=12, dtype=torch.bfloat16)
+    ref = fused64(A, B, Act.GELU, bias, aux, AuxOp.ADD)
+    got = _fused(A, B, OutType.BF16, Act.GELU, bias, OutType.F32, aux, OutType.BF16, AuxOp.ADD)
+    check_rounded(got, *ref, OutType.BF16, want)
+    again = _fused(A, B, OutType.BF16, Act.GELU, bias, OutType.F32, aux, OutType.BF16, AuxOp.ADD)
+    assert torch.equal(got, again)
+    # without a workspace: whole tiles, the same tolerance
+    got = _fused(A, B, OutType.BF16, Act.GELU, bias, OutType.F32, aux, OutType.BF16, AuxOp.ADD, ws=False)
+    check_rounded(got, *ref, OutType.BF16, want + " without workspace")
+
+
+@pytest.mark.parametrize("M,N,K,want", [(1, 128, 128, None), (33, 384, 160, None), (130, 512, 2048, None),
+                                        (17, 2048, 4096, "splits"), (2050, 6144, 512, None), (1500, 2048, 24576, "banded")])
+def test_quantised_output(M, N, K, want):
+    if want:
+        r = _route_of(OutType.F16, M, N, K)
+        assert r["splits"] > 1 and (want == "splits" or r[want]), r
+    A, B = Operand(M, K, 1.0, 13), Operand(N, K, K ** -0.5, 14)
+    bias, aux = _randn(N, seed=15), _randn(M, N, seed=16)
+    bias[32:64] = -1e4  # a block that ReLU makes all zero: scale code 127
+    rb = N * 3 // 4 + 32
+    packed = torch.full((M + 1, rb), 0x5A, dtype=torch.uint8, device="cuda")
+    scales = torch.full((lib.tiled_scale_bytes(M, N),), 0x5A, dtype=torch.uint8, device="cuda")
+    w, n = _workspace(A, N)
+    ep = lib.Epilogue(bias, OutType.F32, Act.RELU, aux, OutType.F32, AuxOp.MUL)
+    rc = lib.gemm_fused_quant(M, N, A.Kp, A.packed, B.packed, A.scales, B.scales, packed, scales, A.row_bytes,
+                              B.row_bytes, ep, w, n, packed_row_bytes=rb)
+    assert rc == lib.OK, lib.last_error_string()
+    _finish()
+    host = packed.cpu().numpy()
+    assert (host[:, N * 3 // 4:] == 0x5A).all() and (host[M] == 0x5A).all()
+    tiled = scales.cpu().numpy()
+    raw = lib.untile_scales(tiled, M, N)
+    filled = tiled.copy()
+    lib_rows = (M + 127) // 128 * 128  # rows past M in the last atom keep what they held
+    if lib_rows > M:
+        rest = lib.untile_scales(filled, lib_rows, N)[M:]
+        assert (rest == 0x5A).all()
+    ref, tol = fused64(A, B, Act.RELU, bias, aux, AuxOp.MUL)
+    if N > 32:
+        assert (raw[:, 1] == 127).all()
+    check_quantised(host[:M], raw, ref, tol, f"{M}x{N}x{K}")
+
+
+# The compact strides of A (0.75*K with K % 128 != 0): re-padded into the workspace, or loaded in place.
+@pytest.mark.parametrize("M,N,K", [(5, 70, 96), (130, 300, 2080), (300, 2056, 480), (513, 520, 800)])
+@pytest.mark.parametrize("ws", [True, False])
+def test_compact_a(M, N, K, ws):
+    A, B = Operand(M, K, 1.0, 17, row_bytes=K * 3 // 4), Operand(N, K, K ** -0.5, 18)
+    got = _fused(A, B, OutType.F16, Act.GELU_TANH, ws=ws)
+    check_rounded(got, *fused64(A, B, Act.GELU_TANH, None, None, AuxOp.NONE), OutType.F16)
+
+
+def test_residual_in_place_and_null_epilogue():
+    A, B = Operand(100, 256, 1.0, 19), Operand(192, 256, 0.06, 20)
+    D = _randn(100, 192, seed=21, dtype=torch.bfloat16)
+    ref, tol = fused64(A, B, Act.NONE, None, D.clone(), AuxOp.ADD)
+    ep = lib.Epilogue(aux=D, aux_type=OutType.BF16, aux_op=AuxOp.ADD)
+    assert lib.gemm_fused(OutType.BF16, 100, 192, 256, A.packed, B.packed, A.scales, B.scales, D, 192, 192, ep) == lib.OK
+    _finish()
+    check_rounded(D, ref, tol, OutType.BF16)
+    plain = torch.empty(128, 256, device="cuda")
+    A, B = Operand(128, 256, 1.0, 22), Operand(256, 256, 0.06, 23)
+    assert lib.gemm_fused(OutType.F32, 128, 256, 256, A.packed, B.packed, A.scales, B.scales, plain, 192, 192) == lib.OK
+    want = torch.empty_like(plain)
+    lib.gemm(OutType.F32, 128, 256, 256, A.packed, B.packed, A.scales, B.scales, want, 192, 192)
+    _finish()
+    assert torch.equal(plain, want)  # a null epilogue is gemm()
+
+
+def test_special_values():
+    A, B = Operand(64, 128, 1.0, 24), Operand(96, 128, 0.1, 25)
+    bias, aux = torch.zeros(96, device="cuda"), torch.zeros(64, 96, device="cuda")
+    bias[0], bias[1], bias[2] = float("inf"), float("-inf"), float("nan")
+    bias[3], bias[4] = 3e38, -3e38
+    aux[5, 10], aux[6, 11] = float("nan"), float("inf")
+    for act in Act:
+        got = _fused(A, B, OutType.F32, act, bias, OutType.F32, aux, OutType.F32, AuxOp.ADD)
+        ref = fused64(A, B, act, bias, aux, AuxOp.ADD)[0]
+        assert got[:, 2].isnan().all() and got[5, 10].isnan() and got[6, 11].isinf()
+        assert (got[:, 0] == float("inf")).all()
+        assert (got[:, 3] > 2e38).all()
+        if act in (Act.RELU,):
+            assert (got[:, 1] == 0).all() and (got[:, 4] == 0).all()
+        fine = ref.isfinite() & (ref.abs() < 1e30)
+        fine[:, 4] = False
+        assert (got[fine].double() - ref[fine]).abs().max() < 1e-4
+
+
+def test_empty_and_stream():
+    A, B = Operand(40, 256, 1.0, 26), Operand(64, 256, 0.06, 27)
+    n0 = lib.launch_count()
+    assert lib.gemm_fused(OutType.F16, 0, 64, 256, 0, 0, 0, 0, 0, 192, 192) == lib.OK
+    assert lib.quantize_device_typed(0, OutType.BF16, 0, 32, 32, 32, 0, 0) == lib.OK
+    assert lib.launch_count() == n0
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        got = _fused(A, B, OutType.F16, stream=s)
+    check_rounded(got, *fused64(A, B, Act.NONE, None, None, AuxOp.NONE), OutType.F16)
+
+
+@pytest.mark.parametrize("rows,cols,ld,padded,offset", [(1, 32, 32, 32, 0), (7, 96, 96, 128, 0), (130, 512, 513, 512, 0),
+                                                        (33, 2080, 2080, 2176, 1), (300, 4160, 4168, 4224, 8),
+                                                        (70000, 32, 32, 128, 0)])
+@pytest.mark.parametrize("ot", list(OutType))
+@pytest.mark.parametrize("tiled", [False, True])
+def test_typed_quantiser(rows, cols, ld, padded, offset, ot, tiled):
+    if tiled and padded % 128:
+        padded = lib.kpad(padded)
+    buf = (_randn(offset + rows * ld, seed=rows + cols) * torch.exp(_randn(offset + rows * ld, seed=2) * 3)).to(DTYPE[ot])
+    x = buf[offset:].view(rows, ld)[:, :cols]
+    x[0, :32] = 0
+    if rows > 4:
+        x[1, 3], x[2, 4], x[3, 5] = float("nan"), float("inf"), float("-inf")
+    full = torch.zeros(rows, padded)
+    full[:, :cols] = x.float().cpu()
+    want = lib.quantize_to_mxfp6(full.numpy())
+    want.scales[:, cols // 32:] = 127
+    packed = torch.full((rows, padded * 3 // 4), 0x5A, dtype=torch.uint8, device="cuda")
+    scales = torch.full((lib.tiled_scale_bytes(rows, padded) if tiled else rows * padded // 32,), 0x5A, dtype=torch.uint8,
+                        device="cuda")
+    assert lib.quantize_device_typed(x, ot, rows, cols, ld, padded, packed, scales, tiled=tiled) == lib.OK
+    torch.cuda.synchronize()
+    assert np.array_equal(packed.cpu().numpy(), want.packed_data)
+    raw = scales.cpu().numpy()
+    raw = lib.untile_scales(raw, rows, padded) if tiled else raw.reshape(rows, -1)
+    assert np.array_equal(raw, want.scales)
+
+
+def _mlp(x, B1, B2, b1, b2, buffers, stream=None):
+    """A feed-forward block as a user runs it: quantise, up with activation to MXFP6, down with residual."""
+    T, H, I = x.shape[0], B1.K, B1.rows
+    xq, sx, hq, sh, y, ws, n = buffers
+    ot = OutType.BF16
+    up = lib.Epilogue(b1, OutType.F32, Act.GELU)
+    down = lib.Epilogue(b2, OutType.F32, aux=x, aux_type=ot, aux_op=AuxOp.ADD)
+    assert lib.quantize_device_typed(x, ot, T, H, H, H, xq, sx, tiled=True, stream=stream) == lib.OK
+    assert lib.gemm_fused_quant(T, I, H, xq, B1.packed, sx, B1.scales, hq, sh, H * 3 // 4, H * 3 // 4, up, ws, n,
+                                stream=stream) == lib.OK
+    assert lib.gemm_fused(ot, T, H, I, hq, B2.packed, sh, B2.scales, y, I * 3 // 4, I * 3 // 4, down, ws, n,
+                          stream=stream) == lib.OK
+
+
+@pytest.mark.parametrize("T,H,I", [(1, 256, 1024), (19, 1024, 4096), (300, 512, 2048)])
+def test_feed_forward_block(T, H, I):
+    """The block's intermediate codes are read back, so each GEMM is held to its own formula; then the
+    block is captured in a graph and replayed on new inputs."""
+    B1, B2 = Operand(I, H, H ** -0.5, 30), Operand(H, I, I ** -0.5, 31)
+    b1, b2 = _randn(I, seed=32, std=0.2), _randn(H, seed=33, std=0.2)
+    x = _randn(T, H, seed=34, dtype=torch.bfloat16)
+    byte = lambda n: torch.zeros(n, dtype=torch.uint8, device="cuda")  # noqa: E731
+    n = max(lib.gemm_fused_workspace_size(T, I, H), lib.gemm_fused_workspace_size(T, H, I))
+    buffers = (byte(T * H * 3 // 4), byte(lib.tiled_scale_bytes(T, H)), byte(T * I * 3 // 4),
+               byte(lib.tiled_scale_bytes(T, I)), torch.empty(T, H, dtype=torch.bfloat16, device="cuda"), byte(n), n)
+
+    def check():
+        _finish()
+        q = lib.quantize_to_mxfp6(x.float().cpu().numpy())
+        a = lib.dequantize_mxfp6(q)
+        A = type("A", (), {"values": torch.from_numpy(a).cuda().double()})
+        packed, raw = buffers[2].cpu().numpy().reshape(T, -1), lib.untile_scales(buffers[3].cpu().numpy(), T, I)
+        check_quantised(packed, raw, *fused64(A, B1, Act.GELU, b1, None, AuxOp.NONE), "hidden")
+        h = lib.QuantizedMatrix(packed, raw, T, I)
+        Hm = type("H", (), {"values": torch.from_numpy(lib.dequantize_mxfp6(h)).cuda().double()})
+        check_rounded(buffers[4], *fused64(Hm, B2, Act.NONE, b2, x, AuxOp.ADD), OutType.BF16, "output")
+
+    _mlp(x, B1, B2, b1, b2, buffers)
+    check()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        _mlp(x, B1, B2, b1, b2, buffers, stream=s)
+    x.copy_(_randn(T, H, seed=35, dtype=torch.bfloat16))
+    g.replay()
+    check()
