@@ -144,6 +144,44 @@ int mxfp6_gemm_fused_quant(int M, int N, int Kp, const void* dA, const void* dBs
  * A_row_bytes is a stride the tensor load cannot address. */
 size_t mxfp6_gemm_fused_workspace_size(int M, int N, int Kp, int A_row_bytes);
 
+/* ---- mixture-of-experts layer for a few tokens -------------------------------------------------
+ * No counterpart in the reference. For 1..128 tokens (a decoding step), where each expert sees too
+ * few tokens to fill a GEMM: every chosen expert's weights are read once.
+ *
+ *   out[t] = [residual[t] +] sum_j weights[t][j] * down_e(h),  h = act(gate_e(x[t])) * up_e(x[t]),
+ *   e = ids[t][j]; without a gate h = act(up_e(x[t]))
+ *
+ * As everywhere in this library both operands of each product are MXFP6: x and h are quantised as by
+ * mxfp6_quantize_device, sums are FP32, and out is rounded once. */
+typedef struct mxfp6_moe_layer {
+    int experts;            /* 1..512 */
+    int hidden, inter;      /* multiples of 128 */
+    int gated;              /* 1: w1 holds each expert's gate rows, then its up rows */
+    int activation;         /* enum mxfp6_activation */
+    const void* w1;         /* packed [experts][(gated ? 2 : 1) * inter][0.75 * hidden] (32-byte aligned) */
+    const uint8_t* s1;      /* its tiled scales, experts * (gated ? 2 : 1) * inter rows (16-byte aligned) */
+    const void* w2;         /* packed [experts][hidden][0.75 * inter] (32-byte aligned) */
+    const uint8_t* s2;      /* its tiled scales, experts * hidden rows (16-byte aligned) */
+} mxfp6_moe_layer;
+
+/* x: [tokens][ldx] of x_type; out, residual (or NULL; may be out itself): of type ot.
+ * Routing, with logits ([tokens][experts] FP32): the top_k (1..16) largest of each token, equal ones
+ * by lowest index; weights are their softmax (renormalize 1) or their share of the softmax over all
+ * experts (0). A logit of -inf or NaN is never chosen; +inf counts as the largest finite value. ids
+ * and weights ([tokens][top_k]; either may be NULL) receive the choice: -1 and 0 where fewer than
+ * top_k experts can be chosen. With logits NULL, ids and weights are inputs: an id outside
+ * [0, experts) is skipped (a token's padding, or another rank's expert), and one expert may be named
+ * twice. A token without any expert gets its residual, or zeros.
+ * tokens 0 launches nothing. The workspace (256-byte aligned, mxfp6_moe_workspace_size bytes, no
+ * initial contents needed) serves one stream at a time. Asynchronous on `stream` (NULL = legacy);
+ * returns an mxfp6_status, which mxfp6_last_error() also reports. */
+int mxfp6_moe(const mxfp6_moe_layer* layer, int ot, int tokens, int top_k, const void* x, int x_type, long long ldx,
+              const float* logits, int renormalize, int* ids, float* weights, const void* residual,
+              long long ld_residual, void* out, long long ldo, void* ws, size_t ws_bytes, void* stream);
+
+/* Workspace bytes of mxfp6_moe; 0 for arguments it refuses. */
+size_t mxfp6_moe_workspace_size(const mxfp6_moe_layer* layer, int tokens, int top_k);
+
 /* CUDA IPC for mxfp6_gemm_gather's peer destinations. export: a 64-byte handle of the
  * allocation holding dptr, and dptr's offset in it. import (in another process, with its own
  * device current): maps the allocation, returns its base (for close) and the pointer. */

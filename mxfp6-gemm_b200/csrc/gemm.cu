@@ -19,6 +19,7 @@
 
 #include "gemm_kernel.cuh"
 #include "gemm_kernel_pair.cuh"
+#include "host.hpp"
 #include "mxfp6/gemm.hpp"
 #include "mxfp6_gemm.h"
 #include "route.hpp"
@@ -110,7 +111,7 @@ EncodeTiledFn encode_fn() {
 // a caller that repeats a call (same buffers, same shape) skips the driver's encode. The key holds
 // every argument that varies; the rest of each encode is fixed per map kind.
 struct TmapKey {
-    int kind;  // 0: FP6 operand, 1: scale atoms, 2: scale atoms read four times (pair B)
+    int kind;  // 0: FP6 operand, 1: scale atoms, 2: scale atoms read four times (pair B), 3: bytes
     int v[4];
     const void* ptr;
     bool operator==(const TmapKey& o) const {
@@ -236,6 +237,36 @@ bool make_sf_tmap_x4(CUtensorMap* map, const void* ptr, int rows, int Kp) {
     const CUresult r = driver_call_in_context([&] {
         return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, const_cast<void*>(ptr), dims, strides, box, estr,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    });
+    if (r != CUDA_SUCCESS) {
+        t_encode_status = (int)r;
+        return false;
+    }
+    t_tmaps.put(k, *map);
+    return true;
+}
+
+// Byte matrix [rows][row_bytes] in 128-byte x box_rows boxes with 128-byte swizzle (operands already in
+// 16-byte slots of 16 codes).
+bool make_bytes_tmap(CUtensorMap* map, const void* ptr, int rows, int row_bytes, int box_rows) {
+    const TmapKey k{3, {rows, row_bytes, box_rows, 0}, ptr};
+    if (const CUtensorMap* hit = t_tmaps.find(k)) {
+        *map = *hit;
+        return true;
+    }
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) {
+        t_encode_status = -1;
+        return false;
+    }
+    cuuint64_t dims[2] = {(cuuint64_t)row_bytes, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)row_bytes};
+    cuuint32_t box[2] = {128u, (cuuint32_t)box_rows};
+    cuuint32_t estr[2] = {1u, 1u};
+    const CUresult r = driver_call_in_context([&] {
+        return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     });
     if (r != CUDA_SUCCESS) {
@@ -941,6 +972,31 @@ void note_launch() {
     g_launches.fetch_add(1, std::memory_order_relaxed);
 }
 
+namespace host {
+void clear() {
+    t_last_error = MXFP6_OK;
+}
+int fail(int code, const char* message) {
+    set_error(code, "%s", message);
+    return code;
+}
+int device() {
+    return current_device();
+}
+int sm_count() {
+    return mxfp6::sm_count();
+}
+long long wait_budget() {
+    return mxfp6::wait_budget();
+}
+bool fp6_tmap(CUtensorMap* map, const void* ptr, int rows, int Kp, int row_bytes, int box_rows) {
+    return make_fp6_tmap(map, ptr, rows, Kp, row_bytes, box_rows);
+}
+bool bytes_tmap(CUtensorMap* map, const void* ptr, int rows, int row_bytes, int box_rows) {
+    return make_bytes_tmap(map, ptr, rows, row_bytes, box_rows);
+}
+}  // namespace host
+
 // ---- C++ API ------------------------------------------------------------------------------------------
 
 TileChoice choose_tile(int M, int N, int Kp) {
@@ -1355,6 +1411,9 @@ int mxfp6_device_status(void) {
     unsigned int v = 0, zero = 0;
     if (cudaMemcpyFromSymbol(&v, g_device_status, sizeof(v)) != cudaSuccess) return -1;
     if (cudaMemcpyToSymbol(g_device_status, &zero, sizeof(zero)) != cudaSuccess) return -1;
+    unsigned int moe = 0;
+    if (!take_moe_status(&moe)) return -1;
+    v |= moe;
     if (v) t_last_error = MXFP6_ERR_DEVICE_TIMEOUT;
     return (int)v;
 }

@@ -80,6 +80,18 @@ _gemm_fused_q = _fn("mxfp6_gemm_fused_quant", C.c_int,
                     [C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int,
                      C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p])
 _ws_fused = _fn("mxfp6_gemm_fused_workspace_size", C.c_size_t, [C.c_int, C.c_int, C.c_int, C.c_int])
+
+
+class _MoEStruct(C.Structure):  # mxfp6_moe_layer
+    _fields_ = [("experts", C.c_int), ("hidden", C.c_int), ("inter", C.c_int), ("gated", C.c_int),
+                ("activation", C.c_int), ("w1", C.c_void_p), ("s1", C.c_void_p), ("w2", C.c_void_p),
+                ("s2", C.c_void_p)]
+
+
+_moe = _fn("mxfp6_moe", C.c_int,
+           [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_int, C.c_longlong, C.c_void_p, C.c_int, C.c_void_p,
+            C.c_void_p, C.c_void_p, C.c_longlong, C.c_void_p, C.c_longlong, C.c_void_p, C.c_size_t, C.c_void_p])
+_ws_moe = _fn("mxfp6_moe_workspace_size", C.c_size_t, [C.c_void_p, C.c_int, C.c_int])
 _ipc_export = _fn("mxfp6_ipc_export", C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(C.c_size_t)])
 _ipc_import = _fn("mxfp6_ipc_import", C.c_int, [C.c_void_p, C.c_size_t, C.POINTER(C.c_void_p),
                                                C.POINTER(C.c_void_p)])
@@ -289,6 +301,34 @@ def gemm_fused_quant(M, N, Kp, dA, dBsh, dsA, dsB, d_packed, d_scales, A_row_byt
 def gemm_fused_workspace_size(M: int, N: int, Kp: int, a_row_bytes: int | None = None) -> int:
     """Workspace bytes of gemm_fused / gemm_fused_quant for an A of row stride a_row_bytes (0.75*Kp)."""
     return _ws_fused(M, N, Kp, Kp * 3 // 4 if a_row_bytes is None else a_row_bytes)
+
+
+class MoELayer:
+    """A mixture-of-experts layer's weights (struct mxfp6_moe_layer): packed w1
+    [experts * (2 if gated else 1) * inter][0.75 * hidden] (each expert's gate rows, then its up rows), packed w2
+    [experts * hidden][0.75 * inter] and their tiled scales, as the GEMM reads them. Keeps them alive."""
+
+    def __init__(self, experts, hidden, inter, w1, s1, w2, s2, gated=True, act=Act.SILU):
+        self.keep = (w1, s1, w2, s2)
+        self.experts, self.hidden, self.inter = experts, hidden, inter
+        self.struct = _MoEStruct(experts, hidden, inter, int(gated), int(act), _addr(w1), _addr(s1), _addr(w2), _addr(s2))
+        self.ref = C.addressof(self.struct)
+
+
+def moe_workspace_size(layer: MoELayer, tokens: int, top_k: int) -> int:
+    """Workspace bytes of moe(); 0 for arguments it refuses."""
+    return _ws_moe(layer.ref, tokens, top_k)
+
+
+def moe(layer, ot, tokens, top_k, x, x_type, out, ws, ws_bytes, logits=None, renormalize=True, ids=None, weights=None,
+        residual=None, ldx=None, ldo=None, ld_residual=None, stream=None) -> int:
+    """mxfp6_moe: a mixture-of-experts layer for up to 128 tokens, routed by logits (ids and weights then
+    receive the choice) or by the given ids and weights. Row strides default to layer.hidden.
+    Asynchronous; returns an mxfp6_status."""
+    H = layer.hidden
+    return _moe(layer.ref, int(ot), tokens, top_k, _addr(x), int(x_type), H if ldx is None else ldx, _addr(logits),
+                int(renormalize), _addr(ids), _addr(weights), _addr(residual), H if ld_residual is None else ld_residual,
+                _addr(out), H if ldo is None else ldo, _addr(ws), ws_bytes, _stream_arg(stream))
 
 
 def ipc_export(t) -> tuple[bytes, int]:
