@@ -9,6 +9,7 @@
 #include <cuda_fp16.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "quant.cuh"
 
@@ -28,7 +29,8 @@ struct Epi {
     uint8_t* scales;    // MXFP6: tiled scales
     long long ld_aux, ldd;
     int bias_type, act, aux_op, aux_type, out_type;
-    int bias_vec, aux_vec, out_vec;  // 16-byte accesses of whole chunks are aligned
+    int aux_vec;            // 16-byte loads of whole aux chunks are aligned
+    int out_vec;            // so are 16-byte (1) or 32-byte (2) stores; 0: neither, or aux is not
     int k_atoms;                     // MXFP6: N / 128
 };
 
@@ -38,10 +40,24 @@ __device__ __forceinline__ float times_sigmoid(float v, float x) {
     return __fdividef(v, 1.0f + __expf(-x));
 }
 
+// v Phi(v) = v (1 - erfc(v / sqrt(2)) / 2) for v >= 0 and v erfc(-v / sqrt(2)) / 2 below, with
+// erfc(x) = (a1 t + ... + a5 t^5) e^(-x^2), t = 1 / (1 + p x) for x >= 0 (Hastings; Abramowitz and Stegun
+// 7.1.26: absolute error 1.5e-7). It has no branch, so a chunk's 32 evaluations overlap.
+__device__ __forceinline__ float gelu_erf(float v) {
+    const float x = fabsf(v) * 0.70710678118654752f;
+    const float t = __fdividef(1.0f, fmaf(0.3275911f, x, 1.0f));
+    float q = fmaf(1.061405429f, t, -1.453152027f);
+    q = fmaf(q, t, 1.421413741f);
+    q = fmaf(q, t, -0.284496736f);
+    q = fmaf(q, t, 0.254829592f);
+    const float half_erfc = 0.5f * q * t * __expf(-x * x);
+    return v * (v < 0.0f ? half_erfc : 1.0f - half_erfc);
+}
+
 __device__ __forceinline__ float activate(int act, float v) {
     switch (act) {
         case ACT_RELU: return v < 0.0f ? 0.0f : v;  // NaN stays NaN
-        case ACT_GELU: return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
+        case ACT_GELU: return gelu_erf(v);
         // 0.5 v (1 + tanh(u)) = v sigmoid(2u), u = sqrt(2/pi) (v + 0.044715 v^3)
         case ACT_GELU_TANH: return times_sigmoid(v, 1.5957691216057308f * (v + 0.044715f * v * v * v));
         case ACT_SILU: return times_sigmoid(v, v);
@@ -130,51 +146,7 @@ __device__ __forceinline__ void load_elems(const void* p, int type, size_t i, in
     }
 }
 
-template <int N>
-__device__ __forceinline__ void store_elems(void* p, int type, size_t i, int valid, bool vec, const float (&v)[N]) {
-    if (vec && valid >= N) {
-        if (type == T_F32) {
-            float4* d = reinterpret_cast<float4*>(static_cast<float*>(p) + i);
-#pragma unroll
-            for (int k = 0; k < N / 4; k++) d[k] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
-        } else {
-            uint4* d = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + i);
-#pragma unroll
-            for (int k = 0; k < N / 8; k++)
-                d[k] = make_uint4(pack2(v[8 * k], v[8 * k + 1], type), pack2(v[8 * k + 2], v[8 * k + 3], type),
-                                  pack2(v[8 * k + 4], v[8 * k + 5], type), pack2(v[8 * k + 6], v[8 * k + 7], type));
-        }
-    } else {
-#pragma unroll
-        for (int k = 0; k < N; k++)
-            if (k < valid) store_elem(p, type, i + k, v[k]);
-    }
-}
-
-// bias, activation and aux on N consecutive accumulators of (row, col..), `valid` of them inside D.
-template <int N>
-__device__ __forceinline__ void epi_apply(const Epi& e, int row, int col, int valid, float (&v)[N]) {
-    if (e.bias) {
-        float b[N];
-        load_elems<N>(e.bias, e.bias_type, (size_t)col, valid, e.bias_vec != 0, b);
-#pragma unroll
-        for (int i = 0; i < N; i++) v[i] += b[i];
-    }
-    activate_all<N>(e.act, v);
-    if (e.aux_op != AUX_NONE) {
-        float a[N];
-        load_elems<N>(e.aux, e.aux_type, (size_t)row * (size_t)e.ld_aux + (size_t)col, valid, e.aux_vec != 0, a);
-        if (e.aux_op == AUX_ADD) {
-#pragma unroll
-            for (int i = 0; i < N; i++) v[i] += a[i];
-        } else {
-#pragma unroll
-            for (int i = 0; i < N; i++) v[i] *= a[i];
-        }
-    }
-}
-
-// The same on four columns (col % 4 == 0) and their store, for the split-K second stage.
+// bias, activation and aux on four columns (col % 4 == 0), and their store, for the split-K second stage.
 __device__ __forceinline__ void epi_apply4(const Epi& e, int row, int col, int valid, float (&v)[4]) {
     if (e.bias) {
 #pragma unroll
@@ -206,15 +178,196 @@ __device__ __forceinline__ void store_elems4(const Epi& e, int row, int col, int
     }
 }
 
-// The whole epilogue of one lane's chunk: accumulators of columns [col, col + 32) of row `row`.
-// `valid` = N - col (> 0); MXFP6 output has N % 128 == 0, so its chunks are whole.
-__device__ __forceinline__ void epi_chunk(const Epi& e, int row, int col, int valid, const uint32_t (&r)[32]) {
+// A warp's copy of a tile's bias in shared memory, CHUNKS chunks of 32 columns `step` columns apart from
+// `col` on: it is loaded while the warp waits for the accumulator, and read back as broadcasts. Loading
+// it from global memory chunk by chunk cost 2.5 us (no activation) to 6 us of 2048 x 6144 x 2048.
+template <int CHUNKS>
+__device__ __forceinline__ void epi_load_bias(const Epi& e, int col, int step, int N, float* bias) {
+    const int lane = threadIdx.x & 31;
+    float v[CHUNKS];
+#pragma unroll
+    for (int i = 0; i < CHUNKS; i++) {
+        const int c = col + i * step + lane;
+        v[i] = e.bias && c < N ? load_elem(e.bias, e.bias_type, (size_t)c) : 0.0f;
+    }
+    __syncwarp();  // the previous tile's reads
+#pragma unroll
+    for (int i = 0; i < CHUNKS; i++) bias[32 * i + lane] = v[i];
+    __syncwarp();
+}
+
+// 8 words as one 32-byte store (full L2 sectors).
+__device__ __forceinline__ void st_v8(void* dst, const uint32_t* w) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                 "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
+
+// NWORDS consecutive words of one row: 256-bit stores where the row is 32-byte aligned, else 128-bit.
+template <int NWORDS>
+__device__ __forceinline__ void store_words(void* dst, const uint32_t* w, bool align32) {
+    if (align32) {
+#pragma unroll
+        for (int i = 0; i < NWORDS / 8; i++) st_v8(static_cast<uint8_t*>(dst) + 32 * i, w + 8 * i);
+    } else {
+        uint4* d = reinterpret_cast<uint4*>(dst);
+#pragma unroll
+        for (int i = 0; i < NWORDS / 4; i++) d[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+    }
+}
+
+// One lane's aux operand of a chunk as loaded (FP32: 32 words, else 16). It is loaded a chunk ahead of
+// its use: the loads of the next chunk are in flight while this one is computed and stored.
+struct AuxRaw {
+    uint4 q[8];
+};
+__device__ __forceinline__ void epi_load_aux(const Epi& e, int row, int col, bool live, AuxRaw& a) {
+    if (e.aux_op == AUX_NONE || !e.aux_vec || !live) return;
+    const size_t i = (size_t)row * (size_t)e.ld_aux + (size_t)col;
+    const uint4* s = e.aux_type == T_F32 ? reinterpret_cast<const uint4*>(static_cast<const float*>(e.aux) + i)
+                                         : reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(e.aux) + i);
+#pragma unroll
+    for (int k = 0; k < 4; k++) a.q[k] = s[k];
+    if (e.aux_type == T_F32) {
+#pragma unroll
+        for (int k = 4; k < 8; k++) a.q[k] = s[k];
+    }
+}
+
+__device__ __forceinline__ void epi_join(int op, float& v, float a) {
+    v = op == AUX_ADD ? v + a : v * a;
+}
+
+// Per epilogue warp: a 32 x 32 FP32 tile of shared memory, rows 36 words apart (16-byte row writes and
+// column reads both spread over all banks).
+constexpr int EPI_TILE_PITCH = 36;
+constexpr int EPI_TILE_BYTES = 32 * EPI_TILE_PITCH * 4;
+
+// The warp's rows of a chunk from its shared-memory tile, lane = column, eight rows at a time.
+// `in`: the lane's column is inside D.
+template <int OT>
+__device__ __forceinline__ void epi_rows(const Epi& e, int row0, int rows, int col, bool in, float bias,
+                                         const float* tile) {
+    using Out = std::conditional_t<OT == T_F32, float, std::conditional_t<OT == T_F16, __half, __nv_bfloat16>>;
+    Out* out = static_cast<Out*>(e.out) + (size_t)row0 * (size_t)e.ldd + (size_t)col;
+    size_t ai = (size_t)row0 * (size_t)e.ld_aux + (size_t)col;
+#pragma unroll 1
+    for (int q = 0; q < rows; q += 8) {
+        float v[8], a[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) a[k] = 0.0f;
+        if (e.aux_op != AUX_NONE) {
+            if (e.aux_type == T_F32) {
+#pragma unroll
+                for (int k = 0; k < 8; k++)
+                    if (in && q + k < rows) a[k] = load_elem(e.aux, T_F32, ai + (size_t)k * (size_t)e.ld_aux);
+            } else if (e.aux_type == T_F16) {
+#pragma unroll
+                for (int k = 0; k < 8; k++)
+                    if (in && q + k < rows) a[k] = load_elem(e.aux, T_F16, ai + (size_t)k * (size_t)e.ld_aux);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; k++)
+                    if (in && q + k < rows) a[k] = load_elem(e.aux, T_BF16, ai + (size_t)k * (size_t)e.ld_aux);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[k] = tile[(q + k) * EPI_TILE_PITCH] + bias;
+        activate_all<8>(e.act, v);
+        if (e.aux_op != AUX_NONE) {
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[k] = e.aux_op == AUX_ADD ? v[k] + a[k] : v[k] * a[k];
+        }
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (in && q + k < rows) store_elem(out + (size_t)k * (size_t)e.ldd, OT, 0, v[k]);
+        out += (size_t)8 * (size_t)e.ldd;
+        ai += (size_t)8 * (size_t)e.ld_aux;
+    }
+}
+
+// The epilogue of a warp's chunk: lane l holds the accumulators of columns [col, col + 32) of row
+// row0 + l. `valid` = N - col (> 0, the same in every lane), `aux` the lane's aux operand when
+// e.aux_vec is set and the chunk is whole, `bias` the chunk's 32 values in shared memory (zeros
+// without a bias), `tile` this warp's.
+//
+// Whole chunks of aligned outputs stay in this layout. Others (odd N, odd pitch, the last columns)
+// go through `tile` to lane = column, so that a store instruction covers consecutive addresses of one
+// row: a per-lane row would touch 32 sectors with each 4-byte store.
+__device__ __forceinline__ void epi_chunk(const Epi& e, int row0, int M, int col, int valid, const uint32_t (&r)[32],
+                                          const AuxRaw& aux, const float* bias, float* tile) {
+    const int lane = threadIdx.x & 31, row = row0 + lane;
+    if (e.out_type != T_MXFP6 && (!e.out_vec || valid < 32)) {
+        const int rows = M - row0 < 32 ? M - row0 : 32;
+        if (rows <= 0) return;
+        uint4* mine = reinterpret_cast<uint4*>(tile + lane * EPI_TILE_PITCH);
+#pragma unroll
+        for (int i = 0; i < 8; i++) mine[i] = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
+        __syncwarp();
+        const bool in = lane < valid;
+        if (e.out_type == T_F32)
+            epi_rows<T_F32>(e, row0, rows, col + lane, in, bias[lane], tile + lane);
+        else if (e.out_type == T_F16)
+            epi_rows<T_F16>(e, row0, rows, col + lane, in, bias[lane], tile + lane);
+        else
+            epi_rows<T_BF16>(e, row0, rows, col + lane, in, bias[lane], tile + lane);
+        __syncwarp();  // the tile is rewritten by the next chunk
+        return;
+    }
+    if (row >= M) return;
     float v[32];
 #pragma unroll
     for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
-    epi_apply<32>(e, row, col, valid, v);
+    if (e.bias) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float4 q = reinterpret_cast<const float4*>(bias)[i];
+            v[4 * i] += q.x;
+            v[4 * i + 1] += q.y;
+            v[4 * i + 2] += q.z;
+            v[4 * i + 3] += q.w;
+        }
+    }
+    activate_all<32>(e.act, v);
+    if (e.aux_op != AUX_NONE) {
+        if (!e.aux_vec) {  // MXFP6 output only
+#pragma unroll
+            for (int i = 0; i < 32; i++)
+                epi_join(e.aux_op, v[i], load_elem(e.aux, e.aux_type, (size_t)row * (size_t)e.ld_aux + (size_t)(col + i)));
+        } else if (e.aux_type == T_F32) {
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                epi_join(e.aux_op, v[4 * k], __uint_as_float(aux.q[k].x));
+                epi_join(e.aux_op, v[4 * k + 1], __uint_as_float(aux.q[k].y));
+                epi_join(e.aux_op, v[4 * k + 2], __uint_as_float(aux.q[k].z));
+                epi_join(e.aux_op, v[4 * k + 3], __uint_as_float(aux.q[k].w));
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const uint32_t w[4] = {aux.q[k].x, aux.q[k].y, aux.q[k].z, aux.q[k].w};
+#pragma unroll
+                for (int h = 0; h < 4; h++) {
+                    float a, b;
+                    unpack2(w[h], e.aux_type, a, b);
+                    epi_join(e.aux_op, v[8 * k + 2 * h], a);
+                    epi_join(e.aux_op, v[8 * k + 2 * h + 1], b);
+                }
+            }
+        }
+    }
+    if (e.out_type == T_F32) {
+        uint32_t w[32];
+#pragma unroll
+        for (int i = 0; i < 32; i++) w[i] = __float_as_uint(v[i]);
+        store_words<32>(static_cast<float*>(e.out) + (size_t)row * (size_t)e.ldd + (size_t)col, w, e.out_vec == 2);
+        return;
+    }
     if (e.out_type != T_MXFP6) {
-        store_elems<32>(e.out, e.out_type, (size_t)row * (size_t)e.ldd + (size_t)col, valid, e.out_vec != 0, v);
+        uint32_t w[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) w[i] = pack2(v[2 * i], v[2 * i + 1], e.out_type);
+        store_words<16>(static_cast<uint16_t*>(e.out) + (size_t)row * (size_t)e.ldd + (size_t)col, w, e.out_vec == 2);
         return;
     }
     float m = 0.0f;

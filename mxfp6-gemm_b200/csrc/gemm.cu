@@ -423,7 +423,6 @@ bool validate_epilogue(const mxfp6_epilogue* ep, int M, int N, kern::Epi& e) {
     }
     e.bias = ep->bias;
     e.bias_type = ep->bias_type;
-    e.bias_vec = aligned(ep->bias, 16);
     e.act = ep->activation;
     return true;
 }
@@ -476,6 +475,7 @@ bool launch_gemm(int M, int N, int Kp, const void* dA, const void* dB, const uin
                  int splits, cudaStream_t stream, const FusedLaunch* fused = nullptr) {
     using C = kern::Config<BN, AMODE>;
     auto kernel = kern::gemm_mxfp6_sm100<BN, OutT, PARTIAL, AMODE>;
+    constexpr int smem_bytes = std::is_same<OutT, kern::FusedOut>::value ? C::FUSED_SMEM_BYTES : C::SMEM_BYTES;
     static std::once_flag attr_once[kMaxDevices];
     const int dev = current_device();
     if (dev < 0 || dev >= kMaxDevices) {
@@ -484,7 +484,7 @@ bool launch_gemm(int M, int N, int Kp, const void* dA, const void* dB, const uin
     }
     cudaError_t attr_err = cudaSuccess;
     std::call_once(attr_once[dev], [&] {
-        attr_err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
+        attr_err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes);
     });
     if (attr_err != cudaSuccess) {
         set_error(MXFP6_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(attr_err));
@@ -524,7 +524,7 @@ bool launch_gemm(int M, int N, int Kp, const void* dA, const void* dB, const uin
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid, 1, 1);
     cfg.blockDim = dim3(kern::threads_for(AMODE), 1, 1);
-    cfg.dynamicSmemBytes = C::SMEM_BYTES;
+    cfg.dynamicSmemBytes = smem_bytes;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     set_pdl(attr[0]);
@@ -550,6 +550,7 @@ bool launch_pair(int M, int N, int Kp, const void* dA, const void* dB, const uin
     auto kernel_lean = kern::gemm_mxfp6_sm100_pair<OutT, PARTIAL, AMODE, kern::EPI_LEAN>;
     auto kernel_sk = kern::gemm_mxfp6_sm100_pair<OutT, PARTIAL, AMODE, PARTIAL ? kern::EPI_LEAN : kern::EPI_STREAM_K>;
     constexpr bool FUSED = std::is_same<OutT, kern::FusedOut>::value;  // one destination, always
+    constexpr int smem_bytes = FUSED ? C::FUSED_SMEM_BYTES : C::SMEM_BYTES;
     auto kernel_all = kern::gemm_mxfp6_sm100_pair<OutT, PARTIAL, AMODE,
                                                   PARTIAL ? kern::EPI_LEAN : FUSED ? kern::EPI_STREAM_K : kern::EPI_ALL>;
     static std::once_flag attr_once[kMaxDevices];
@@ -562,7 +563,7 @@ bool launch_pair(int M, int N, int Kp, const void* dA, const void* dB, const uin
     std::call_once(attr_once[dev], [&] {
         for (auto k : {kernel_lean, kernel_sk, kernel_all})
             if (attr_err == cudaSuccess)
-                attr_err = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
+                attr_err = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes);
     });
     if (attr_err != cudaSuccess) {
         set_error(MXFP6_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(attr_err));
@@ -617,8 +618,8 @@ bool launch_pair(int M, int N, int Kp, const void* dA, const void* dB, const uin
     p.band_n = banded ? band->n : 0;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2 * clusters, 1, 1);
-    cfg.blockDim = dim3(kern::threads_for(AMODE), 1, 1);
-    cfg.dynamicSmemBytes = C::SMEM_BYTES;
+    cfg.blockDim = dim3(kern::pair_threads<OutT, AMODE>(), 1, 1);
+    cfg.dynamicSmemBytes = smem_bytes;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1283,7 +1284,10 @@ int mxfp6_gemm_fused(int ot, int M, int N, int Kp, const void* dA, const void* d
     f.epi.out = dD;
     f.epi.ldd = ldd;
     f.epi.out_type = ot;
-    f.epi.out_vec = aligned(dD, 16) && (M == 1 || ldd * esize % 16 == 0);
+    f.epi.out_vec = f.epi.aux_op != kern::AUX_NONE && !f.epi.aux_vec        ? 0
+                    : aligned(dD, 32) && (M == 1 || ldd * esize % 32 == 0) ? 2
+                    : aligned(dD, 16) && (M == 1 || ldd * esize % 16 == 0) ? 1
+                                                                          : 0;
     run_validated(ot, M, N, Kp, dA, dBsh, dsA, dsB, kern::DstList{}, A_row_bytes, B_row_bytes, ws, ws_bytes,
                   static_cast<cudaStream_t>(stream), &f);
     return t_last_error;

@@ -73,7 +73,8 @@ struct Config {
     static constexpr int TMEM_COLS = BN == 256 ? 512 : 256;
     static constexpr int BAR_BYTES = 256;
     static constexpr int SMEM_BYTES = 1024 + STAGES * (AB_STAGE + SF_STAGE) + BAR_BYTES;
-    static_assert(SMEM_BYTES <= 227 * 1024, "shared memory budget");
+    static constexpr int FUSED_SMEM_BYTES = SMEM_BYTES + 4 * (EPI_TILE_BYTES + BN * 4);  // fused: tiles, biases
+    static_assert(FUSED_SMEM_BYTES <= 227 * 1024, "shared memory budget");
 };
 
 // Output destinations: D is written into each of n row-major [M][ldd] matrices at column col0
@@ -151,26 +152,6 @@ __device__ __forceinline__ TileCoord decode_tile(int t, const Params& p) {
 __device__ __forceinline__ void raise_status(unsigned int bit, volatile int* abort_flag) {
     atomicOr(&g_device_status, bit);
     *abort_flag = 1;
-}
-
-// 32 consecutive outputs of one row from 32 FP32 accumulator words. With a 32-byte aligned
-// destination the stores are 256-bit (full L2 sectors), otherwise 128-bit.
-__device__ __forceinline__ void st_v8(void* dst, const uint32_t* w) {
-    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]),
-                 "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
-                 : "memory");
-}
-
-template <int NWORDS>
-__device__ __forceinline__ void store_words(void* dst, const uint32_t* w, bool align32) {
-    if (align32) {
-#pragma unroll
-        for (int i = 0; i < NWORDS / 8; i++) st_v8(static_cast<uint8_t*>(dst) + 32 * i, w + 8 * i);
-    } else {
-        uint4* d = reinterpret_cast<uint4*>(dst);
-#pragma unroll
-        for (int i = 0; i < NWORDS / 4; i++) d[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-    }
 }
 
 // 32 FP32 accumulator words of one row -> OutT words (RNE): 32 words for float, 16 for half
@@ -256,6 +237,7 @@ __global__ void __launch_bounds__(threads_for(AMODE), 1)
                      const ParamsFor<OutT> p) {
     using C = Config<BN, AMODE>;
     constexpr bool COMPACT = AMODE != A_TMA;
+    constexpr bool FUSED = std::is_same<OutT, FusedOut>::value;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     // 1024-byte alignment for the 128-byte-swizzled operand tiles.
     const uint32_t raw_u32 = sm100::smem_u32(smem_raw);
@@ -442,25 +424,34 @@ __global__ void __launch_bounds__(threads_for(AMODE), 1)
         uint32_t acc_phase = 0;
         for (int t = blockIdx.x; t < total_tiles; t += gridDim.x) {
             const TileCoord tc = decode_tile(t, p);
+            const int row = tc.mb * BM + 32 * quarter + lane;
+            const int col0 = tc.nb * BN;
+            [[maybe_unused]] AuxRaw aux[2];
+            [[maybe_unused]] float* tile = reinterpret_cast<float*>(bar_ptr + C::BAR_BYTES + quarter * (EPI_TILE_BYTES + BN * 4));
+            if constexpr (FUSED) {
+                epi_load_aux(p.epi, row, col0, row < p.M && col0 + 32 <= p.N, aux[0]);
+                epi_load_bias<BN / 32>(p.epi, col0, 32, p.N, tile + EPI_TILE_BYTES / 4);
+            }
             if (!sm100::wait_parity_bounded(acc_full, acc_phase, abort_flag, p.wait_budget)) {
                 if (!*abort_flag) raise_status(0x4u, abort_flag);
                 break;
             }
             sm100::tc_fence_after();
-            const int row = tc.mb * BM + 32 * quarter + lane;
-            const int col0 = tc.nb * BN;
 #pragma unroll 1
             for (int c = 0; c < BN; c += 32) {
                 if (col0 + c >= p.N) break;  // masked half tile (uniform across the warp)
                 uint32_t r[32];
                 sm100::tmem_ld_32x32b_x32(t_row + (uint32_t)c, r);
                 sm100::tmem_ld_wait(r);
-                if (row < p.M) {
+                if constexpr (FUSED) {
+                    aux[1] = aux[0];
+                    epi_load_aux(p.epi, row, col0 + c + 32, row < p.M && c + 32 < BN && col0 + c + 64 <= p.N, aux[0]);
+                    epi_chunk(p.epi, row - lane, p.M, col0 + c, p.N - col0 - c, r, aux[1], tile + EPI_TILE_BYTES / 4 + c,
+                              tile);
+                } else if (row < p.M) {
                     if constexpr (PARTIAL) {
                         float* dst = p.ws + ((size_t)tc.split * p.M + row) * p.N + col0 + c;
                         store_words<32>(dst, r, p.out_align32 != 0);
-                    } else if constexpr (std::is_same<OutT, FusedOut>::value) {
-                        epi_chunk(p.epi, row, col0 + c, p.N - col0 - c, r);
                     } else {
                         uint32_t w[ChunkWords<OutT>::N];
                         convert_chunk<OutT>(r, w);

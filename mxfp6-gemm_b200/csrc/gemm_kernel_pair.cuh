@@ -63,12 +63,27 @@ struct PairConfig {
     static constexpr int TMEM_SFB = 480;  // B scales: 8 columns (8-column aligned for the wide copy)
     static constexpr int TMEM_SFA = 488;  // A scales: 4 columns
     static_assert(TMEM_SFA + 4 <= 512, "tensor memory budget");
-    static constexpr int EPI_WARPS = 4;
     static constexpr int BAR_BYTES = 256;
     static constexpr int SK_TILE_FLOATS = BM * BN;  // one hand-off slot: a 256 x 256 FP32 accumulator
     static constexpr int SMEM_BYTES = 1024 + STAGES * (AB_STAGE + SF_STAGE) + BAR_BYTES + EPI_STG_BYTES;
-    static_assert(SMEM_BYTES <= 227 * 1024, "shared memory budget");
+    // A fused epilogue (with the tensor load's A) has two warps per lane quarter, which take its
+    // chunks in turn: one warp per scheduler leaves the activation's latencies exposed. Each has a
+    // tile and its chunks' biases in shared memory.
+    static constexpr int FUSED_HALVES = AMODE == A_TMA ? 2 : 1;
+    static constexpr int FUSED_EPI_WARP = EPI_TILE_BYTES + BN / FUSED_HALVES * 4;
+    static constexpr int FUSED_SMEM_BYTES =
+        SMEM_BYTES - EPI_STG_BYTES + 4 * FUSED_HALVES * FUSED_EPI_WARP;
+    static_assert(SMEM_BYTES <= 227 * 1024 && FUSED_SMEM_BYTES <= 227 * 1024, "shared memory budget");
 };
+
+template <typename OutT, int AMODE>
+__host__ __device__ constexpr int pair_epilogue_halves() {
+    return std::is_same<OutT, FusedOut>::value ? PairConfig<AMODE>::FUSED_HALVES : 1;
+}
+template <typename OutT, int AMODE>
+__host__ __device__ constexpr int pair_threads() {
+    return threads_for(AMODE) + 128 * (pair_epilogue_halves<OutT, AMODE>() - 1);
+}
 
 __device__ __forceinline__ void store_cluster_u32(uint32_t cluster_addr, uint32_t v) {
     asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
@@ -201,13 +216,18 @@ __device__ __forceinline__ PairUnit pair_unit(const Params& p, const PairWork& w
 // 2-11% slower on shapes that never ran it.
 constexpr int EPI_LEAN = 0, EPI_STREAM_K = 1, EPI_ALL = 2;
 template <typename OutT, bool PARTIAL, int AMODE = A_TMA, int EPI = EPI_ALL>
-__global__ void __launch_bounds__(threads_for(AMODE), 1)
+__global__ void __launch_bounds__(pair_threads<OutT, AMODE>(), 1)
     gemm_mxfp6_sm100_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                           const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB,
                           const ParamsFor<OutT> p) {
     using C = PairConfig<AMODE>;
     constexpr bool COMPACT = AMODE != A_TMA;
+    constexpr bool FUSED = std::is_same<OutT, FusedOut>::value;
     static_assert(C::SUB == 1, "one 128-deep slab per stage");
+    // Epilogue warps per lane quarter; half h takes the chunks whose place in the reading order is
+    // h modulo HALVES, in filling a taken-over accumulator as in reading one.
+    constexpr int HALVES = pair_epilogue_halves<OutT, AMODE>();
+    constexpr int EPI_WARPS = 4 * HALVES;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     const uint32_t raw_u32 = sm100::smem_u32(smem_raw);
     const uint32_t base = (raw_u32 + 1023u) & ~1023u;
@@ -254,12 +274,12 @@ __global__ void __launch_bounds__(threads_for(AMODE), 1)
         }
         for (int b = 0; b < 2; b++) {
             sm100::mbar_init(acc_full0 + 8u * b, 1);
-            sm100::mbar_init(acc_empty0 + 8u * b, 2 * C::EPI_WARPS);
+            sm100::mbar_init(acc_empty0 + 8u * b, 2 * EPI_WARPS);
         }
-        sm100::mbar_init(ovl_free, 2 * C::EPI_WARPS);
+        sm100::mbar_init(ovl_free, 2 * 4);  // the warps that read the shared chunk
         sm100::mbar_init(drain_bar, 1);
-        sm100::mbar_init(fill_bar, 2 * C::EPI_WARPS);
-        sm100::mbar_init(handed_bar, C::EPI_WARPS);
+        sm100::mbar_init(fill_bar, 2 * EPI_WARPS);
+        sm100::mbar_init(handed_bar, EPI_WARPS);
         *abort_flag = 0;
         sm100::fence_mbar_init();
         sm100::fence_async_shared();
@@ -465,7 +485,7 @@ __global__ void __launch_bounds__(threads_for(AMODE), 1)
         sm100::cp_async_wait_all();
     } else {
         // ---------------- epilogue (warps 2..5 of both CTAs) ----------------
-        const int quarter = warp & 3;
+        const int quarter = warp & 3, half = HALVES > 1 ? (warp - EPI_WARP0) / 4 : 0;
         const uint32_t t_lane = tmem_base + ((uint32_t)(32 * quarter) << 16);
         const uint32_t leader_acc_empty = sm100::mapa_shared(acc_empty0, 0);
         const uint32_t leader_ovl_free = sm100::mapa_shared(ovl_free, 0);
@@ -497,6 +517,7 @@ __global__ void __launch_bounds__(threads_for(AMODE), 1)
 #pragma unroll 1
             for (int c = 0; c < C::BN / 32; c++) {
                 if (!((c == shared_chunk ? FILL_SHARED : FILL_REST) & part)) continue;
+                if (HALVES > 1 && (bb ? c : C::BN / 32 - 1 - c) % HALVES != half) continue;
                 uint32_t r[32];
 #pragma unroll
                 for (int q = 0; q < 8; q++) {
@@ -545,6 +566,16 @@ __global__ void __launch_bounds__(threads_for(AMODE), 1)
             const int row = tc.mb * C::BM + tile_row;
             const int col0 = tc.nb * C::BN;
             const bool regroup = XG && !hand_off && p.dst.n > 1;
+            [[maybe_unused]] AuxRaw aux[2];
+            [[maybe_unused]] float* tile =
+                reinterpret_cast<float*>(epi_stg + (quarter + 4 * half) * (FUSED ? C::FUSED_EPI_WARP : 0));
+            if constexpr (FUSED) {
+                if (!hand_off) {
+                    const int fcol = col0 + 32 * (b ? half : C::BN / 32 - 1 - half);
+                    epi_load_aux(p.epi, row, fcol, row < p.M && fcol + 32 <= p.N, aux[0]);
+                    epi_load_bias<C::BN / 32 / HALVES>(p.epi, fcol, (b ? 32 : -32) * HALVES, p.N, tile + EPI_TILE_BYTES / 4);
+                }
+            }
             // The whole warp waits (a suspended wait takes no issue slots), so it is still converged
             // when the accumulator completes. Measured on B200: 1.7% on cfg2 against one polling
             // lane and a shuffle.
@@ -558,17 +589,19 @@ __global__ void __launch_bounds__(threads_for(AMODE), 1)
             sm100::tc_fence_after();
             uint32_t pend[16];  // FP16/BF16 with several destinations: first chunk of a 64-column pair
 #pragma unroll 1
-            for (int j = 0; j < C::BN / 32; j++) {
+            for (int j = half; j < C::BN / 32; j += HALVES) {
                 // buffer 0 top-down, buffer 1 bottom-up: the shared chunk [224, 256) goes first
                 const int c = b ? j : (C::BN / 32 - 1 - j);
                 const uint32_t tcol = (b ? C::BUF1_COL : 0) + 32 * c;
                 uint32_t r[32];
                 sm100::tmem_ld_32x32b_x32(t_lane + tcol, r);
                 sm100::tmem_ld_wait(r);
-                if (j == 0) {
-                    sm100::tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) sm100::mbar_arrive_remote(leader_ovl_free);
+                if (j == half) {
+                    if (half == 0) {
+                        sm100::tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) sm100::mbar_arrive_remote(leader_ovl_free);
+                    }
                     if (early) take_over(pair_unit<XF>(p, work, cluster_id, num_clusters, ui + 1), b ^ 1, FILL_SHARED);
                 }
                 const int col = col0 + 32 * c;
@@ -602,11 +635,16 @@ __global__ void __launch_bounds__(threads_for(AMODE), 1)
                             }
                         }
                     }
+                } else if constexpr (FUSED) {
+                    aux[1] = aux[0];
+                    const int ncol = col + (b ? 32 : -32) * HALVES;  // the warp's next chunk
+                    epi_load_aux(p.epi, row, ncol, row < p.M && j + HALVES < C::BN / 32 && ncol + 32 <= p.N, aux[0]);
+                    if (col < p.N)
+                        epi_chunk(p.epi, row - lane, p.M, col, p.N - col, r, aux[1],
+                                  tile + EPI_TILE_BYTES / 4 + j / HALVES * 32, tile);
                 } else if (row < p.M && col < p.N) {
                     if constexpr (PARTIAL) {
                         store_words<32>(p.ws + ((size_t)tc.split * p.M + row) * p.N + col, r, p.out_align32 != 0);
-                    } else if constexpr (std::is_same<OutT, FusedOut>::value) {
-                        epi_chunk(p.epi, row, col, p.N - col, r);
                     } else {
                         uint32_t w[ChunkWords<OutT>::N];
                         convert_chunk<OutT>(r, w);
