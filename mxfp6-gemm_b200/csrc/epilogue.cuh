@@ -370,14 +370,13 @@ __device__ __forceinline__ void epi_chunk(const Epi& e, int row0, int M, int col
         store_words<16>(static_cast<uint16_t*>(e.out) + (size_t)row * (size_t)e.ldd + (size_t)col, w, e.out_vec == 2);
         return;
     }
-    float m = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 32; i++) m = fmaxf(m, fabsf(v[i]));
-    const uint32_t code = scale_code(m);
+    bool nan0, nan1;
+    const float m0 = max_abs16(v, nan0), m1 = max_abs16(v + 16, nan1);
+    const uint32_t code = scale_code(fmaxf(m0, m1));
     const float inv = e8m0_reciprocal(code);
     uint32_t w[6];
-    quantize16(v, inv, w[0], w[1], w[2]);
-    quantize16(v + 16, inv, w[3], w[4], w[5]);
+    quantize16(v, inv, nan0, w[0], w[1], w[2]);
+    quantize16(v + 16, inv, nan1, w[3], w[4], w[5]);
     uint2* d = reinterpret_cast<uint2*>(static_cast<uint8_t*>(e.out) + (size_t)row * (size_t)e.ldd + (size_t)(col / 4 * 3));
     d[0] = make_uint2(w[0], w[1]);
     d[1] = make_uint2(w[2], w[3]);

@@ -207,13 +207,12 @@ __global__ void __launch_bounds__(PREP_THREADS) moe_prep(const PrepParams p) {
         const int esize = p.x_type == kern::T_F32 ? 4 : 2;
         const bool vec = ((reinterpret_cast<uintptr_t>(p.x) | (uintptr_t)(p.ldx * esize)) & 15) == 0;
         if (live) kern::load_elems<16>(p.x, p.x_type, (size_t)t * (size_t)p.ldx + (size_t)col, 16, vec, v);
-        float m = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 16; i++) m = fmaxf(m, fabsf(v[i]));
+        bool nan;
+        float m = max_abs16(v, nan);
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
         const uint32_t code = scale_code(m);
         uint32_t w0, w1, w2;
-        quantize16(v, e8m0_reciprocal(code), w0, w1, w2);
+        quantize16(v, e8m0_reciprocal(code), nan, w0, w1, w2);
         if (!live) continue;
         for (int j = 0; j < K; j++) {
             const int i = t * K + j, e = s_id[i];
@@ -479,13 +478,12 @@ __global__ void __launch_bounds__(ProductConfig<KIND, NMAX>::THREADS, ProductCon
                                 v[4 * i + 3] *= q.w;
                             }
                         }
-                        float m = 0.0f;
-#pragma unroll
-                        for (int i = 0; i < 16; i++) m = fmaxf(m, fabsf(v[i]));
+                        bool nan;
+                        float m = max_abs16(v, nan);
                         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
                         const uint32_t code = scale_code(m);
                         uint32_t w0, w1, w2;
-                        quantize16(v, e8m0_reciprocal(code), w0, w1, w2);
+                        quantize16(v, e8m0_reciprocal(code), nan, w0, w1, w2);
                         const int rk = c0 + c, col = tile * ROWS + 16 * g;
                         if (rk < en.n) {
                             *reinterpret_cast<uint4*>(p.hq + (size_t)(en.start + rk) * p.inter + col) =

@@ -18,6 +18,7 @@
 
 #include "mxfp6_gemm.h"
 #include "epilogue.cuh"
+#include "host.hpp"
 #include "quant.cuh"
 #include "sm100_ptx.cuh"
 
@@ -28,10 +29,6 @@ namespace {
 
 template <typename T>
 struct TypeOf;
-template <>
-struct TypeOf<float> {
-    static constexpr int value = kern::T_F32;
-};
 template <>
 struct TypeOf<__half> {
     static constexpr int value = kern::T_F16;
@@ -70,14 +67,12 @@ __global__ void __launch_bounds__(256) quantize_kernel(const float* __restrict__
 #pragma unroll
         for (int i = 0; i < 16; i++) v[i] = 0.0f;
     }
-    float m = 0.0f;  // fmaxf returns the other operand for a NaN: NaN never wins the max
-#pragma unroll
-    for (int i = 0; i < 16; i++) m = fmaxf(m, fabsf(v[i]));
+    bool nan;
+    float m = max_abs16(v, nan);
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
     const uint32_t code = scale_code(m);
-    const float inv = e8m0_reciprocal(code);
     uint32_t w0, w1, w2;
-    quantize16(v, inv, w0, w1, w2);
+    quantize16(v, e8m0_reciprocal(code), nan, w0, w1, w2);
     if (live) {
         uint32_t* dst = reinterpret_cast<uint32_t*>(packed + (size_t)row * out_row_bytes + (size_t)col / 4 * 3);
         dst[0] = w0;
@@ -97,11 +92,48 @@ __global__ void __launch_bounds__(256) quantize_kernel(const float* __restrict__
     }
 }
 
-// The quantiser for any input type and row stride, padding in the same pass: the lane layout of
-// quantize_kernel, with rows as a grid-stride loop and the tail [cols, padded_cols) written as zero
-// codes with the finite scale 127. HBM bound: a BF16 element reads 2 bytes and writes 0.78.
-// VEC: 16-byte aligned rows (ld and base), so a lane's 16 values are two (four for FP32) wide loads.
+// A lane's 16 values as loaded.
+template <typename In>
+struct Raw16 {
+    uint4 q[sizeof(In)];  // 16 * sizeof(In) bytes
+};
 template <typename In, bool VEC>
+__device__ __forceinline__ void load_raw(const In* src, Raw16<In>& r) {
+    if constexpr (VEC) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(In); i++) r.q[i] = __ldg(reinterpret_cast<const uint4*>(src) + i);
+    } else {
+        In* d = reinterpret_cast<In*>(r.q);
+#pragma unroll
+        for (int i = 0; i < 16; i++) d[i] = src[i];
+    }
+}
+__device__ __forceinline__ void raw_values(const Raw16<float>& r, float (&v)[16]) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        v[4 * i] = __uint_as_float(r.q[i].x);
+        v[4 * i + 1] = __uint_as_float(r.q[i].y);
+        v[4 * i + 2] = __uint_as_float(r.q[i].z);
+        v[4 * i + 3] = __uint_as_float(r.q[i].w);
+    }
+}
+template <typename In>
+__device__ __forceinline__ void raw_values(const Raw16<In>& r, float (&v)[16]) {
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        kern::unpack2(r.q[i].x, TypeOf<In>::value, v[8 * i], v[8 * i + 1]);
+        kern::unpack2(r.q[i].y, TypeOf<In>::value, v[8 * i + 2], v[8 * i + 3]);
+        kern::unpack2(r.q[i].z, TypeOf<In>::value, v[8 * i + 4], v[8 * i + 5]);
+        kern::unpack2(r.q[i].w, TypeOf<In>::value, v[8 * i + 6], v[8 * i + 7]);
+    }
+}
+
+// The quantiser for any input type and row stride, padding in the same pass: the lane layout of
+// quantize_kernel, with the tail [cols, padded_cols) written as zero codes with the finite scale 127. A
+// BF16 element reads 2 bytes and writes 0.78, so the instructions per element count as much as the bytes: a warp
+// takes its 512 columns of ROWS consecutive rows, all loads first, and sets up its addresses once.
+// VEC: 16-byte aligned rows (ld and base), so a lane's 16 values are two (four for FP32) wide loads.
+template <typename In, bool VEC, int ROWS>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const In* __restrict__ in, int rows, int cols, long long ld,
                                                             int padded_cols, uint8_t* __restrict__ packed,
                                                             uint8_t* __restrict__ scales, int tiled) {
@@ -114,28 +146,39 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const In* __restrict
     const bool live = col < cols;  // cols % 32 == 0: a lane's 16 values are all in or all out
     const bool kept = col < padded_cols;
     const size_t out_row_bytes = (size_t)(padded_cols / 4 * 3);
-    for (int row = blockIdx.y; row < rows; row += gridDim.y) {
-        float v[16];
+    const int j = col / 32;
+    for (int row0 = blockIdx.y * ROWS; row0 < rows; row0 += gridDim.y * ROWS) {
+        const In* src = in + (size_t)row0 * (size_t)ld + (size_t)col;
+        Raw16<In> raw[ROWS];
 #pragma unroll
-        for (int i = 0; i < 16; i++) v[i] = 0.0f;
-        if (live) kern::load_elems<16>(in, TypeOf<In>::value, (size_t)row * (size_t)ld + (size_t)col, 16, VEC, v);
-        float m = 0.0f;  // fmaxf returns the other operand for a NaN: NaN never wins the max
+        for (int i = 0; i < ROWS; i++) {
 #pragma unroll
-        for (int i = 0; i < 16; i++) m = fmaxf(m, fabsf(v[i]));
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-        const uint32_t code = scale_code(m);
-        uint32_t w0, w1, w2;
-        quantize16(v, e8m0_reciprocal(code), w0, w1, w2);
-        if (!kept) continue;
-        uint32_t* dst = reinterpret_cast<uint32_t*>(packed + (size_t)row * out_row_bytes + (size_t)(col / 4 * 3));
-        dst[0] = w0;
-        dst[1] = w1;
-        dst[2] = w2;
-        if ((lane & 1) == 0) {
-            const int j = col / 32;
-            const size_t off = tiled ? scale_atom_offset(row, j, padded_cols / 128)
-                                     : (size_t)row * (size_t)(padded_cols / 32) + (size_t)j;
-            scales[off] = (uint8_t)code;
+            for (int k = 0; k < (int)sizeof(In); k++) raw[i].q[k] = make_uint4(0u, 0u, 0u, 0u);
+            if (live && row0 + i < rows) load_raw<In, VEC>(src, raw[i]);
+            src += ld;
+        }
+        uint8_t* dst = packed + (size_t)row0 * out_row_bytes + (size_t)(col / 4 * 3);
+#pragma unroll
+        for (int i = 0; i < ROWS; i++) {
+            float v[16];
+            raw_values(raw[i], v);
+            bool nan;
+            float m = max_abs16(v, nan);
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+            const uint32_t code = scale_code(m);
+            uint32_t w0, w1, w2;
+            quantize16(v, e8m0_reciprocal(code), nan, w0, w1, w2);
+            if (kept && row0 + i < rows) {
+                reinterpret_cast<uint32_t*>(dst)[0] = w0;
+                reinterpret_cast<uint32_t*>(dst)[1] = w1;
+                reinterpret_cast<uint32_t*>(dst)[2] = w2;
+                if ((lane & 1) == 0) {
+                    const size_t off = tiled ? scale_atom_offset(row0 + i, j, padded_cols / 128)
+                                             : (size_t)(row0 + i) * (size_t)(padded_cols / 32) + (size_t)j;
+                    scales[off] = (uint8_t)code;
+                }
+            }
+            dst += out_row_bytes;
         }
     }
 }
@@ -192,12 +235,13 @@ __global__ void __launch_bounds__(256) repad_kernel(const uint8_t* __restrict__ 
 
 }  // namespace
 
-template <typename In>
-cudaError_t launch_quantize_rows(const In* in, int rows, int cols, long long ld, int padded_cols, uint8_t* packed,
-                                 uint8_t* scales, int tiled, cudaStream_t stream) {
+template <typename In, int ROWS>
+cudaError_t launch_quantize_rows_of(const In* in, int rows, int cols, long long ld, int padded_cols, uint8_t* packed,
+                                    uint8_t* scales, int tiled, cudaStream_t stream) {
     const bool vec = (reinterpret_cast<uintptr_t>(in) & 15) == 0 && (rows == 1 || ld * (long long)sizeof(In) % 16 == 0);
+    const int groups = (rows + ROWS - 1) / ROWS;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((padded_cols + 4095) / 4096), (unsigned)(rows < 65535 ? rows : 65535), 1);
+    cfg.gridDim = dim3((unsigned)((padded_cols + 4095) / 4096), (unsigned)(groups < 65535 ? groups : 65535), 1);
     cfg.blockDim = dim3(256, 1, 1);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -205,10 +249,21 @@ cudaError_t launch_quantize_rows(const In* in, int rows, int cols, long long ld,
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return vec ? cudaLaunchKernelEx(&cfg, quantize_rows_kernel<In, true>, in, rows, cols, ld, padded_cols, packed, scales,
-                                    tiled)
-               : cudaLaunchKernelEx(&cfg, quantize_rows_kernel<In, false>, in, rows, cols, ld, padded_cols, packed,
+    return vec ? cudaLaunchKernelEx(&cfg, quantize_rows_kernel<In, true, ROWS>, in, rows, cols, ld, padded_cols, packed,
+                                    scales, tiled)
+               : cudaLaunchKernelEx(&cfg, quantize_rows_kernel<In, false, ROWS>, in, rows, cols, ld, padded_cols, packed,
                                     scales, tiled);
+}
+
+// Rows per warp: four (two of FP32: the same registers) once that still fills the GPU's warps, else one.
+template <typename In>
+cudaError_t launch_quantize_rows(const In* in, int rows, int cols, long long ld, int padded_cols, uint8_t* packed,
+                                 uint8_t* scales, int tiled, cudaStream_t stream) {
+    constexpr int MANY = sizeof(In) == 4 ? 2 : 4;
+    const long long warps = (long long)rows * ((padded_cols + 511) / 512);
+    if (warps >= (long long)host::sm_count() * 48 * MANY)
+        return launch_quantize_rows_of<In, MANY>(in, rows, cols, ld, padded_cols, packed, scales, tiled, stream);
+    return launch_quantize_rows_of<In, 1>(in, rows, cols, ld, padded_cols, packed, scales, tiled, stream);
 }
 
 // Launch the re-pad copy with the widest unit the pointers and strides allow (used by

@@ -199,7 +199,7 @@ def test_empty_and_stream():
 
 @pytest.mark.parametrize("rows,cols,ld,padded,offset", [(1, 32, 32, 32, 0), (7, 96, 96, 128, 0), (130, 512, 513, 512, 0),
                                                         (33, 2080, 2080, 2176, 1), (300, 4160, 4168, 4224, 8),
-                                                        (70000, 32, 32, 128, 0)])
+                                                        (70000, 32, 32, 128, 0), (30001, 64, 72, 64, 0), (3003, 4160, 4161, 4224, 1)])
 @pytest.mark.parametrize("ot", list(OutType))
 @pytest.mark.parametrize("tiled", [False, True])
 def test_typed_quantiser(rows, cols, ld, padded, offset, ot, tiled):
