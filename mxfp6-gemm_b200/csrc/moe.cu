@@ -65,17 +65,22 @@ bool valid_layer(const mxfp6_moe_layer* l) {
 // Programmatic stream serialization: each kernel of the chain sets up while the one before it finishes, and
 // touches global memory only after griddepcontrol.wait.
 template <typename... KArgs, typename... Args>
-cudaError_t launch(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, cudaStream_t stream, Args... args) {
+cudaError_t launch(void (*kernel)(KArgs...), dim3 grid, int cluster, int threads, size_t smem, cudaStream_t stream,
+                   Args... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads, 1, 1);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)cluster;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
     if (e == cudaSuccess) note_launch();
     return e;
@@ -94,7 +99,7 @@ cudaError_t launch_product(const CUtensorMap& tmW, const CUtensorMap& tmB, const
     });
     if (attr_err[dev] != cudaSuccess) return attr_err[dev];
     const long long slots = (long long)host::sm_count() * C::CTAS;
-    return launch(kernel, dim3((unsigned)(items < slots ? items : slots)), C::THREADS, C::SMEM_BYTES, stream, tmW, tmB, p);
+    return launch(kernel, dim3((unsigned)(items < slots ? items : slots)), 1, C::THREADS, C::SMEM_BYTES, stream, tmW, tmB, p);
 }
 
 template <int KIND>
@@ -204,9 +209,12 @@ extern "C" int mxfp6_moe(const mxfp6_moe_layer* layer, int ot, int tokens, int t
     pp.slot_w = reinterpret_cast<float*>(b + w.slot_w);
     pp.xq = b + w.xq;
     pp.sx = b + w.sx;
-    const int units = tokens * ((H + 511) / 512), per = moe::PREP_THREADS / 32;
-    int prep_grid = (units + per - 1) / per;
-    if (prep_grid > host::sm_count()) prep_grid = host::sm_count();
+    // eight 512-column chunks a CTA: more would wait for one another's issue slots, and the routing that every CTA
+    // repeats takes its full width anyway
+    int prep_grid = (tokens * ((H + 511) / 512) + 7) / 8;
+    if (prep_grid > 32) prep_grid = 32;
+    const int cluster = logits && tokens > 16 ? 8 : 1;
+    prep_grid = (prep_grid + cluster - 1) / cluster * cluster;
 
     moe::ProductParams up;
     up.sW = layer->s1;
@@ -245,12 +253,14 @@ extern "C" int mxfp6_moe(const mxfp6_moe_layer* layer, int ot, int tokens, int t
     cp.out_vec = aligned(out, 16) && (tokens == 1 || ldo * (long long)oe % 16 == 0);
 
     const long long max_up = (long long)w.max_entries * up.tiles, max_down = (long long)w.max_entries * down.tiles;
-    cudaError_t e = launch(moe::moe_prep, dim3(prep_grid), moe::PREP_THREADS, 0, st, pp);
+    const int E = layer->experts;
+    auto prep = E <= 64 ? moe::moe_prep<2> : E <= 128 ? moe::moe_prep<4> : E <= 256 ? moe::moe_prep<8> : moe::moe_prep<16>;
+    cudaError_t e = launch(prep, dim3(prep_grid), cluster, moe::PREP_THREADS, 0, st, pp);
     if (e == cudaSuccess)
         e = layer->gated ? launch_product_for<moe::KIND_UP_GATED>(w.nmax, tmW1, tmX, up, max_up, st)
                          : launch_product_for<moe::KIND_UP>(w.nmax, tmW1, tmX, up, max_up, st);
     if (e == cudaSuccess) e = launch_product_for<moe::KIND_DOWN>(w.nmax, tmW2, tmH, down, max_down, st);
-    if (e == cudaSuccess) e = launch(moe::moe_combine, dim3((H + 1023) / 1024, tokens), 256, 0, st, cp);
+    if (e == cudaSuccess) e = launch(moe::moe_combine, dim3((H + 1023) / 1024, tokens), 1, 256, 0, st, cp);
     if (e != cudaSuccess) {
         cudaGetLastError();
         std::snprintf(msg, sizeof(msg), "moe launch failed: %s", cudaGetErrorString(e));

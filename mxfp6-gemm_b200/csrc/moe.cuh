@@ -11,8 +11,8 @@
 //                into one row per (token, choice), sorted by expert, so that an expert's tokens are consecutive
 //                rows and the products need no gather.
 //   moe_product  the two products, weights as the 128-row MMA operand (tcgen05.mma kind::mxf8f6f4, M = 128) and
-//                the expert's tokens as the N = 16..128 one: up (gate and up rows interleaved 64 + 64 in a tile, so
-//                that one CTA holds both halves of each hidden value and quantises them) and down.
+//                the expert's tokens as the N = 16..128 one: up (64 gate and 64 up rows in a tile, so that one CTA
+//                holds both halves of each hidden value and quantises them) and down.
 //   moe_combine  the weighted sum over each token's choices, in their order.
 //
 // All FP32 sums are in tensor memory or registers, in a fixed order: results do not depend on timing.
@@ -72,157 +72,219 @@ __device__ __forceinline__ float key_logit(uint32_t k) {
 
 constexpr int PREP_THREADS = 1024;
 
-// Every CTA routes all tokens for itself (a warp per token; at most 4 rounds of MAX_TOPK warp reductions) and
-// sorts the choices by expert in shared memory; no CTA waits for another. Then the grid's warps share out the
-// 512-column chunks of x. CTA 0 writes the tables and the chosen ids and weights.
+// Every cluster of CTAs (one CTA, or eight for many tokens) routes all tokens for itself, a warp per token, and every CTA
+// sorts the choices by expert in shared memory; no cluster waits for another. Then the grid's warps share out the 512-column chunks of x, whose
+// loads were issued first. CTA 0 writes the tables and the chosen ids and weights. PER: experts per lane (2, 4, 8, 16).
+template <int PER>
 __global__ void __launch_bounds__(PREP_THREADS) moe_prep(const PrepParams p) {
-    __shared__ short s_id[MAX_SLOTS];
-    __shared__ float s_w[MAX_SLOTS];
-    __shared__ short s_rank[MAX_SLOTS];
+    __shared__ short s_id[MAX_SLOTS], s_rank[MAX_SLOTS];
     __shared__ int s_count[MAX_EXPERTS], s_start[MAX_EXPERTS], s_entry[MAX_EXPERTS];
+    __shared__ __align__(4) uint8_t s_hits[MAX_SLOTS / 32 * MAX_EXPERTS];  // choices of an expert among 32 slots
+    int* s_place = reinterpret_cast<int*>(s_hits);  // then, per slot: entry * 128 + row inside the entry
     sm100::griddep_launch_dependents();
     sm100::griddep_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr int WARPS = PREP_THREADS / 32;
-    const int T = p.tokens, K = p.top_k, E = p.experts, slots = T * K;
+    const int T = p.tokens, K = p.top_k, E = p.experts, slots = T * K, nmax_log = 31 - __clz(p.nmax);
+    const int chunks = (p.hidden + 511) / 512, k_slabs = p.hidden / 128, units = T * chunks;
+    const bool vec =
+        ((reinterpret_cast<uintptr_t>(p.x) | (uintptr_t)(p.ldx * (p.x_type == kern::T_F32 ? 4 : 2))) & 15) == 0;
+    // 16 columns of a unit (token, chunk) per lane
+    auto load_unit = [&](int u, float(&v)[16]) {
+        const int t = u / chunks, col = (u - t * chunks) * 512 + 16 * lane;
+#pragma unroll
+        for (int i = 0; i < 16; i++) v[i] = 0.0f;
+        if (u < units && col < p.hidden)
+            kern::load_elems<16>(p.x, p.x_type, (size_t)t * (size_t)p.ldx + (size_t)col, 16, vec, v);
+    };
+    float v[16];
+    int u = warp * gridDim.x + blockIdx.x;
+    load_unit(u, v);
 
+    const int groups = (slots + 31) / 32;
+    const int ctas = (int)sm100::cluster_nctarank(), rank = (int)sm100::cluster_ctarank(), first = rank + ctas * warp;
+    for (int i = threadIdx.x; i < (groups * E + 3) / 4; i += PREP_THREADS) reinterpret_cast<uint32_t*>(s_hits)[i] = 0;
     if (p.logits) {
-        constexpr int PER = MAX_EXPERTS / 32;
-        for (int t = warp; t < T; t += WARPS) {
-            uint32_t key[PER];
+        uint32_t next[PER];
+        auto load_keys = [&](int t) {
 #pragma unroll
             for (int i = 0; i < PER; i++) {
                 const int e = lane + 32 * i;
-                key[i] = e < E ? logit_key(p.logits[(size_t)t * E + e]) : 0u;
+                next[i] = t < T && e < E ? logit_key(p.logits[(size_t)t * E + e]) : 0u;
             }
-            float top = 0.0f, sum = 0.0f, mine = 0.0f;  // lane j keeps choice j's exponential
-            int chosen = -1;
+        };
+        load_keys(first);
+        for (int t = first; t < T; t += ctas * WARPS) {
+            uint32_t key[PER];
+#pragma unroll
+            for (int i = 0; i < PER; i++) key[i] = next[i];
+            load_keys(t + ctas * WARPS);
+            short* ids = s_id + t * K;
+            if (lane < K) ids[lane] = -1;
+            __syncwarp();
+            uint32_t top = 0, mine = 0;  // lane j keeps choice j
+            float sum = 0.0f;
             for (int j = 0; j < K; j++) {
                 uint32_t best = 0;
-                int at = 0;
+                int e = lane;
 #pragma unroll
                 for (int i = 0; i < PER; i++)
                     if (key[i] > best) {
                         best = key[i];
-                        at = i;
+                        e = lane + 32 * i;
                     }
                 const uint32_t all = __reduce_max_sync(0xffffffffu, best);
                 if (all == 0) break;  // nothing left to choose
-                const int e = __reduce_min_sync(0xffffffffu, best == all ? lane + 32 * at : 0x7fffffff);
+                bool win = best == all;
+                const uint32_t ties = __ballot_sync(0xffffffffu, win);
+                if (ties & (ties - 1)) {  // equal logits in several lanes: the lowest index (every lane takes part)
+                    const int lowest = __reduce_min_sync(0xffffffffu, win ? e : 0x7fffffff);
+                    win = win && e == lowest;
+                }
                 if (j == 0) {
-                    top = key_logit(all);
+                    top = all;
                     if (!p.renormalize) {  // softmax over every expert
-                        float s = 0.0f;
 #pragma unroll
                         for (int i = 0; i < PER; i++)
-                            if (key[i]) s += expf(key_logit(key[i]) - top);
+                            if (key[i]) sum += expf(key_logit(key[i]) - key_logit(top));
 #pragma unroll
-                        for (int d = 16; d > 0; d /= 2) s += __shfl_xor_sync(0xffffffffu, s, d);
-                        sum = s;
+                        for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
                     }
                 }
-                const float ex = expf(key_logit(all) - top);
-                if (p.renormalize) sum += ex;
-                if (lane == j) {
-                    mine = ex;
-                    chosen = e;
-                }
+                if (lane == j) mine = all;
+                if (win) ids[j] = (short)e;
 #pragma unroll
                 for (int i = 0; i < PER; i++)
-                    if (lane + 32 * i == e) key[i] = 0;
+                    if (win && lane + 32 * i == e) key[i] = 0;
             }
-            if (lane < K) {
-                s_id[t * K + lane] = (short)chosen;
-                s_w[t * K + lane] = chosen >= 0 ? mine / sum : 0.0f;
+            if ((int)blockIdx.x < ctas) {
+                const float x = mine ? expf(key_logit(mine) - key_logit(top)) : 0.0f;
+                if (p.renormalize) {
+                    sum = x;
+#pragma unroll
+                    for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+                }
+                __syncwarp();
+                if (lane < K) {
+                    const float w = mine ? x / sum : 0.0f;
+                    p.slot_w[t * K + lane] = w;
+                    if (p.ids) p.ids[t * K + lane] = ids[lane];
+                    if (p.weights) p.weights[t * K + lane] = w;
+                }
             }
+        }
+        if (ctas > 1) {  // the other CTAs' tokens
+            __syncwarp();
+            sm100::cluster_sync();
+            for (int i = threadIdx.x; i < slots; i += PREP_THREADS) {
+                const uint32_t owner = (uint32_t)((i / K) % ctas);
+                if ((int)owner == rank) continue;
+                uint16_t id;
+                asm volatile("ld.shared::cluster.u16 %0, [%1];"
+                             : "=h"(id)
+                             : "r"(sm100::mapa_shared(sm100::smem_u32(s_id + i), owner))
+                             : "memory");
+                s_id[i] = (short)id;
+            }
+            asm volatile("barrier.cluster.arrive.release;" ::: "memory");
         }
     } else {
         for (int i = threadIdx.x; i < slots; i += PREP_THREADS) {
             const int e = p.ids[i];
             s_id[i] = (short)(e >= 0 && e < E ? e : -1);
-            s_w[i] = p.weights[i];
+            if (blockIdx.x == 0) p.slot_w[i] = p.weights[i];
         }
     }
     __syncthreads();
-    // count and rank each expert's choices in (token, choice) order: a warp per expert
-    for (int e = warp; e < E; e += WARPS) {
+    // rank of each choice among its expert's, in (token, choice) order: within 32 slots, then over those before
+    for (int g = warp; g < groups; g += WARPS) {
+        const int i = 32 * g + lane, e = i < slots ? s_id[i] : -1;
+        const uint32_t same = __match_any_sync(0xffffffffu, e);
+        const int before = __popc(same & ((1u << lane) - 1u));
+        if (e >= 0) {
+            s_rank[i] = (short)before;
+            if (before == 0) s_hits[g * E + e] = (uint8_t)__popc(same);
+        }
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < E; e += PREP_THREADS) {
         int n = 0;
-        for (int i0 = 0; i0 < slots; i0 += 32) {
-            const bool hit = i0 + lane < slots && s_id[i0 + lane] == e;
-            const uint32_t b = __ballot_sync(0xffffffffu, hit);
-            if (hit) s_rank[i0 + lane] = (short)(n + __popc(b & ((1u << lane) - 1u)));
-            n += __popc(b);
-        }
-        if (lane == 0) s_count[e] = n;
+        for (int g = 0; g < groups; g++) n += s_hits[g * E + e];
+        s_count[e] = n;
+    }
+    for (int i = threadIdx.x; i < slots; i += PREP_THREADS) {
+        const int e = s_id[i];
+        int n = s_rank[i];
+        if (e >= 0)
+            for (int g = 0; g < i / 32; g++) n += s_hits[g * E + e];
+        s_rank[i] = (short)n;
     }
     __syncthreads();
-    if (warp == 0) {  // first row and first entry of each expert
-        int start = 0, entry = 0;
-        for (int e0 = 0; e0 < E; e0 += 32) {
-            const int n = e0 + lane < E ? s_count[e0 + lane] : 0;
-            const int m = (n + p.nmax - 1) / p.nmax;
-            int sn = n, se = m;
+    if (warp == 0) {  // first row and first entry of each expert: PER consecutive experts a lane, then over the lanes
+        int n[PER], sn = 0, se = 0;
 #pragma unroll
-            for (int d = 1; d < 32; d *= 2) {
-                const int a = __shfl_up_sync(0xffffffffu, sn, d), b = __shfl_up_sync(0xffffffffu, se, d);
-                if (lane >= d) {
-                    sn += a;
-                    se += b;
-                }
-            }
-            if (e0 + lane < E) {
-                s_start[e0 + lane] = start + sn - n;
-                s_entry[e0 + lane] = entry + se - m;
-                if (blockIdx.x == 0)
-                    for (int c = 0; c < m; c++)
-                        p.entries[entry + se - m + c] =
-                            Entry{e0 + lane, start + sn - n + c * p.nmax, min(n - c * p.nmax, p.nmax), 0};
-            }
-            start += __shfl_sync(0xffffffffu, sn, 31);
-            entry += __shfl_sync(0xffffffffu, se, 31);
+        for (int i = 0; i < PER; i++) {
+            const int e = lane * PER + i;
+            n[i] = e < E ? s_count[e] : 0;
+            sn += n[i];
+            se += (n[i] + p.nmax - 1) >> nmax_log;
         }
-        if (blockIdx.x == 0 && lane == 0) *p.n_entries = entry;
+        int start = sn, entry = se;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const int a = __shfl_up_sync(0xffffffffu, start, d), b = __shfl_up_sync(0xffffffffu, entry, d);
+            if (lane >= d) {
+                start += a;
+                entry += b;
+            }
+        }
+        if (blockIdx.x == 0 && lane == 31) *p.n_entries = entry;
+        start -= sn;
+        entry -= se;
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            const int e = lane * PER + i;
+            if (e < E) {
+                s_start[e] = start;
+                s_entry[e] = entry;
+            }
+            if (blockIdx.x == 0)
+                for (int c = 0; c < n[i]; c += p.nmax, entry++)
+                    p.entries[entry] = Entry{e, start + c, min(n[i] - c, p.nmax), 0};
+            else
+                entry += (n[i] + p.nmax - 1) >> nmax_log;
+            start += n[i];
+        }
     }
     __syncthreads();
-    if (blockIdx.x == 0) {
-        for (int i = threadIdx.x; i < slots; i += PREP_THREADS) {
-            const int e = s_id[i];
-            p.slot_of[i] = e < 0 ? -1 : s_start[e] + s_rank[i];
-            p.slot_w[i] = s_w[i];
-            if (p.logits) {
-                if (p.ids) p.ids[i] = e;
-                if (p.weights) p.weights[i] = s_w[i];
-            }
-        }
+    if (p.logits && ctas > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");  // s_id was read
+    for (int i = threadIdx.x; i < slots; i += PREP_THREADS) {
+        const int e = s_id[i], at = s_rank[i];
+        const int row = e < 0 ? -1 : s_start[e] + at;
+        if (blockIdx.x == 0) p.slot_of[i] = row;
+        s_id[i] = (short)row;  // from here on the sorted row, and the entry with the row inside it
+        s_place[i] = e < 0 ? 0 : (s_entry[e] + (at >> nmax_log)) * 128 + (at & (p.nmax - 1));
     }
-    // x, in chunks of 512 columns: a lane quantises 16 values (one block per lane pair) and writes them to
-    // each of its token's rows
-    const int chunks = (p.hidden + 511) / 512, k_slabs = p.hidden / 128;
-    for (int u = blockIdx.x * WARPS + warp; u < T * chunks; u += gridDim.x * WARPS) {
+    __syncthreads();
+    // a lane quantises its 16 values (one block per lane pair) and writes them to each of its token's rows
+    for (; u < units; u += gridDim.x * WARPS) {
         const int t = u / chunks, col = (u - t * chunks) * 512 + 16 * lane;
-        const bool live = col < p.hidden;
-        float v[16];
-#pragma unroll
-        for (int i = 0; i < 16; i++) v[i] = 0.0f;
-        const int esize = p.x_type == kern::T_F32 ? 4 : 2;
-        const bool vec = ((reinterpret_cast<uintptr_t>(p.x) | (uintptr_t)(p.ldx * esize)) & 15) == 0;
-        if (live) kern::load_elems<16>(p.x, p.x_type, (size_t)t * (size_t)p.ldx + (size_t)col, 16, vec, v);
         bool nan;
         float m = max_abs16(v, nan);
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
         const uint32_t code = scale_code(m);
         uint32_t w0, w1, w2;
         quantize16(v, e8m0_reciprocal(code), nan, w0, w1, w2);
-        if (!live) continue;
+        load_unit(u + gridDim.x * WARPS, v);
+        if (col >= p.hidden) continue;
+#pragma unroll 4
         for (int j = 0; j < K; j++) {
-            const int i = t * K + j, e = s_id[i];
-            if (e < 0) continue;
-            const int rank = s_rank[i], row = s_start[e] + rank, r = rank % p.nmax;
+            const int row = s_id[t * K + j], place = s_place[t * K + j], r = place & 127;
+            if (row < 0) continue;
             *reinterpret_cast<uint4*>(p.xq + (size_t)row * p.hidden + col) = make_uint4(w0, w1, w2, 0u);
-            if ((lane & 1) == 0) {
-                const size_t atom = (size_t)(s_entry[e] + rank / p.nmax) * k_slabs + col / 128;
-                p.sx[atom * 512 + (r % 32) * 16 + (r / 32) * 4 + (col / 32) % 4] = (uint8_t)code;
-            }
+            if ((lane & 1) == 0)
+                p.sx[((size_t)(place >> 7) * k_slabs + col / 128) * 512 + (r % 32) * 16 + (r / 32) * 4 + (col / 32) % 4] =
+                    (uint8_t)code;
         }
     }
 }

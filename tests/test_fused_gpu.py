@@ -108,7 +108,7 @@ def test_schedules(M, N, K, want):
 
 
 @pytest.mark.parametrize("M,N,K,want", [(1, 128, 128, None), (33, 384, 160, None), (130, 512, 2048, None),
-                                        (17, 2048, 4096, "splits"), (2050, 6144, 512, None), (1500, 2048, 24576, "banded")])
+                                        (17, 2048, 4096, None), (64, 128, 256, None), (128, 640, 384, None), (200, 2048, 4096, "splits"), (2050, 6144, 512, None), (1500, 2048, 24576, "banded")])
 def test_quantised_output(M, N, K, want):
     if want:
         r = _route_of(OutType.F16, M, N, K)
