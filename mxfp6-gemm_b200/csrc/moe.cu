@@ -254,7 +254,8 @@ extern "C" int mxfp6_moe(const mxfp6_moe_layer* layer, int ot, int tokens, int t
 
     const long long max_up = (long long)w.max_entries * up.tiles, max_down = (long long)w.max_entries * down.tiles;
     const int E = layer->experts;
-    auto prep = E <= 64 ? moe::moe_prep<2> : E <= 128 ? moe::moe_prep<4> : E <= 256 ? moe::moe_prep<8> : moe::moe_prep<16>;
+    const bool few = w.slots <= moe::FEW && (!logits || moe::route_by_rank(tokens, E, renormalize));
+    auto prep = few ? moe::moe_prep_few : E <= 64 ? moe::moe_prep<2> : E <= 128 ? moe::moe_prep<4> : E <= 256 ? moe::moe_prep<8> : moe::moe_prep<16>;
     cudaError_t e = launch(prep, dim3(prep_grid), cluster, moe::PREP_THREADS, 0, st, pp);
     if (e == cudaSuccess)
         e = layer->gated ? launch_product_for<moe::KIND_UP_GATED>(w.nmax, tmW1, tmX, up, max_up, st)

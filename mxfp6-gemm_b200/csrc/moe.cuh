@@ -72,6 +72,144 @@ __device__ __forceinline__ float key_logit(uint32_t k) {
 
 constexpr int PREP_THREADS = 1024;
 
+// Routing by counting: a thread per (token, expert) counts the experts that come before its own (larger logit, or equal
+// and lower index), which is its place in the choice. E comparisons a thread, but no chain of reductions. For one token
+// of 64 experts with 8 choices 1.6 us less than a warp's eight rounds of moe_prep; with a thread's work growing with E and
+// every thread busy it no longer is (61 tokens of 64 experts: 0.9 us more).
+constexpr int RANK_KEYS = PREP_THREADS;
+inline bool route_by_rank(int tokens, int experts, int renormalize) {
+    return renormalize && tokens * experts <= RANK_KEYS && experts <= 128;
+}
+// s_id [T][K] gets the choices, s_ex [T][K] their exponentials. Ends with a barrier.
+__device__ __forceinline__ void choose_by_rank(const PrepParams& p, uint32_t* s_key, short* s_id, float* s_ex) {
+    const int E = p.experts, K = p.top_k, t = threadIdx.x / E, e = threadIdx.x - t * E;
+    const uint32_t key = t < p.tokens ? logit_key(p.logits[(size_t)t * E + e]) : 0u;
+    s_key[threadIdx.x] = key;
+    if (threadIdx.x < p.tokens * K) {
+        s_id[threadIdx.x] = -1;
+        s_ex[threadIdx.x] = 0.0f;
+    }
+    __syncthreads();
+    if (key) {
+        const uint32_t* row = s_key + t * E;
+        int before = 0;
+        uint32_t top = 0;
+#pragma unroll 8
+        for (int i = 0; i < E; i++) {
+            const uint32_t other = row[i];
+            before += other > key || (other == key && i < e) ? 1 : 0;
+            top = max(top, other);
+        }
+        if (before < K) {
+            s_id[t * K + before] = (short)e;
+            s_ex[t * K + before] = expf(key_logit(key) - key_logit(top));
+        }
+    }
+    __syncthreads();
+}
+// Their softmax, in the order of the choices, to the workspace and the caller's ids and weights: a warp per token.
+__device__ __forceinline__ void write_by_rank(const PrepParams& p, const short* s_id, const float* s_ex) {
+    const int K = p.top_k, lane = threadIdx.x & 31;
+    for (int t = threadIdx.x >> 5; t < p.tokens; t += PREP_THREADS / 32) {
+        const float x = lane < K ? s_ex[t * K + lane] : 0.0f;
+        float sum = x;
+#pragma unroll
+        for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        if (lane < K) {
+            const int id = s_id[t * K + lane];
+            const float w = id >= 0 ? x / sum : 0.0f;
+            p.slot_w[t * K + lane] = w;
+            if (p.ids) p.ids[t * K + lane] = id;
+            if (p.weights) p.weights[t * K + lane] = w;
+        }
+    }
+}
+
+// 16 columns of a unit (token, 512-column chunk) of x per lane; zeros past the last unit and column.
+__device__ __forceinline__ void load_unit(const PrepParams& p, int u, int units, int chunks, bool vec, float (&v)[16]) {
+    const int t = u / chunks, col = (u - t * chunks) * 512 + 16 * (threadIdx.x & 31);
+#pragma unroll
+    for (int i = 0; i < 16; i++) v[i] = 0.0f;
+    if (u < units && col < p.hidden)
+        kern::load_elems<16>(p.x, p.x_type, (size_t)t * (size_t)p.ldx + (size_t)col, 16, vec, v);
+}
+__device__ __forceinline__ bool wide_rows(const PrepParams& p) {
+    return ((reinterpret_cast<uintptr_t>(p.x) | (uintptr_t)(p.ldx * (p.x_type == kern::T_F32 ? 4 : 2))) & 15) == 0;
+}
+// Write 16 codes and (even lanes) their block's scale to sorted row `row`, row `r` of entry `entry`.
+__device__ __forceinline__ void store_unit(const PrepParams& p, int row, int entry, int r, int col, uint4 codes,
+                                           uint32_t scale) {
+    *reinterpret_cast<uint4*>(p.xq + (size_t)row * p.hidden + col) = codes;
+    if ((threadIdx.x & 1) == 0)
+        p.sx[((size_t)entry * (p.hidden / 128) + col / 128) * 512 + (r % 32) * 16 + (r / 32) * 4 + (col / 32) % 4] =
+            (uint8_t)scale;
+}
+
+constexpr int FEW = 32;
+// At most FEW choices in all, given or routed by rank (a decoding step of one to a few tokens, where latency is all):
+// every warp keeps the sorted list in its lanes, a lane per choice, and no barrier follows the choice.
+__global__ void __launch_bounds__(PREP_THREADS) moe_prep_few(const PrepParams p) {
+    __shared__ uint32_t s_key[RANK_KEYS];
+    __shared__ float s_ex[FEW];
+    __shared__ short s_id[FEW];
+    sm100::griddep_launch_dependents();
+    sm100::griddep_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int T = p.tokens, K = p.top_k, E = p.experts, slots = T * K, nmax_log = 31 - __clz(p.nmax);
+    const int chunks = (p.hidden + 511) / 512, units = T * chunks;
+    const bool vec = wide_rows(p);
+    float v[16];
+    int u = warp * gridDim.x + blockIdx.x;
+    load_unit(p, u, units, chunks, vec, v);
+    if (p.logits) {
+        choose_by_rank(p, s_key, s_id, s_ex);
+        if (blockIdx.x == 0) write_by_rank(p, s_id, s_ex);
+    } else {
+        if (threadIdx.x < slots) {
+            const int e = p.ids[threadIdx.x];
+            s_id[threadIdx.x] = (short)(e >= 0 && e < E ? e : -1);
+            if (blockIdx.x == 0) p.slot_w[threadIdx.x] = p.weights[threadIdx.x];
+        }
+        __syncthreads();
+    }
+    // lane i holds choice i: its rank among its expert's, the first row and the first entry of that expert
+    const int e = lane < slots ? s_id[lane] : -1;
+    const uint32_t same = __match_any_sync(0xffffffffu, e);
+    const int rank = __popc(same & ((1u << lane) - 1u)), n = __popc(same);
+    const int m = e >= 0 && rank == 0 ? (n + p.nmax - 1) >> nmax_log : 0;  // entries, at the expert's first choice
+    int start = 0, entry = 0, total = 0;
+    for (int i = 0; i < slots; i++) {
+        const int ei = __shfl_sync(0xffffffffu, e, i), mi = __shfl_sync(0xffffffffu, m, i);
+        total += mi;
+        if (ei >= 0 && ei < e) {
+            start++;
+            entry += mi;
+        }
+    }
+    if (blockIdx.x == 0 && warp == 0) {
+        if (lane == 0) *p.n_entries = total;
+        for (int c = 0; c < m; c++) p.entries[entry + c] = Entry{e, start + (c << nmax_log), min(n - (c << nmax_log), p.nmax), 0};
+        if (lane < slots) p.slot_of[lane] = e < 0 ? -1 : start + rank;
+    }
+    const int row = e < 0 ? -1 : start + rank;
+    entry += rank >> nmax_log;
+    for (; u < units; u += gridDim.x * (PREP_THREADS / 32)) {
+        const int t = u / chunks, col = (u - t * chunks) * 512 + 16 * lane;
+        bool nan;
+        float top = max_abs16(v, nan);
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        const uint32_t code = scale_code(top);
+        uint32_t w0, w1, w2;
+        quantize16(v, e8m0_reciprocal(code), nan, w0, w1, w2);
+        load_unit(p, u + gridDim.x * (PREP_THREADS / 32), units, chunks, vec, v);
+        for (int j = 0; j < K; j++) {
+            const int to = __shfl_sync(0xffffffffu, row, t * K + j), en = __shfl_sync(0xffffffffu, entry, t * K + j);
+            const int r = __shfl_sync(0xffffffffu, rank, t * K + j) & (p.nmax - 1);
+            if (to >= 0 && col < p.hidden) store_unit(p, to, en, r, col, make_uint4(w0, w1, w2, 0u), code);
+        }
+    }
+}
+
 // Every cluster of CTAs (one CTA, or eight for many tokens) routes all tokens for itself, a warp per token, and every CTA
 // sorts the choices by expert in shared memory; no cluster waits for another. Then the grid's warps share out the 512-column chunks of x, whose
 // loads were issued first. CTA 0 writes the tables and the chosen ids and weights. PER: experts per lane (2, 4, 8, 16).
@@ -86,20 +224,11 @@ __global__ void __launch_bounds__(PREP_THREADS) moe_prep(const PrepParams p) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr int WARPS = PREP_THREADS / 32;
     const int T = p.tokens, K = p.top_k, E = p.experts, slots = T * K, nmax_log = 31 - __clz(p.nmax);
-    const int chunks = (p.hidden + 511) / 512, k_slabs = p.hidden / 128, units = T * chunks;
-    const bool vec =
-        ((reinterpret_cast<uintptr_t>(p.x) | (uintptr_t)(p.ldx * (p.x_type == kern::T_F32 ? 4 : 2))) & 15) == 0;
-    // 16 columns of a unit (token, chunk) per lane
-    auto load_unit = [&](int u, float(&v)[16]) {
-        const int t = u / chunks, col = (u - t * chunks) * 512 + 16 * lane;
-#pragma unroll
-        for (int i = 0; i < 16; i++) v[i] = 0.0f;
-        if (u < units && col < p.hidden)
-            kern::load_elems<16>(p.x, p.x_type, (size_t)t * (size_t)p.ldx + (size_t)col, 16, vec, v);
-    };
+    const int chunks = (p.hidden + 511) / 512, units = T * chunks;
+    const bool vec = wide_rows(p);
     float v[16];
     int u = warp * gridDim.x + blockIdx.x;
-    load_unit(u, v);
+    load_unit(p, u, units, chunks, vec, v);
 
     const int groups = (slots + 31) / 32;
     const int ctas = (int)sm100::cluster_nctarank(), rank = (int)sm100::cluster_ctarank(), first = rank + ctas * warp;
@@ -173,27 +302,27 @@ __global__ void __launch_bounds__(PREP_THREADS) moe_prep(const PrepParams p) {
                 }
             }
         }
-        if (ctas > 1) {  // the other CTAs' tokens
-            __syncwarp();
-            sm100::cluster_sync();
-            for (int i = threadIdx.x; i < slots; i += PREP_THREADS) {
-                const uint32_t owner = (uint32_t)((i / K) % ctas);
-                if ((int)owner == rank) continue;
-                uint16_t id;
-                asm volatile("ld.shared::cluster.u16 %0, [%1];"
-                             : "=h"(id)
-                             : "r"(sm100::mapa_shared(sm100::smem_u32(s_id + i), owner))
-                             : "memory");
-                s_id[i] = (short)id;
-            }
-            asm volatile("barrier.cluster.arrive.release;" ::: "memory");
-        }
     } else {
         for (int i = threadIdx.x; i < slots; i += PREP_THREADS) {
             const int e = p.ids[i];
             s_id[i] = (short)(e >= 0 && e < E ? e : -1);
             if (blockIdx.x == 0) p.slot_w[i] = p.weights[i];
         }
+    }
+    if (p.logits && ctas > 1) {  // the other CTAs' tokens
+        __syncwarp();
+        sm100::cluster_sync();
+        for (int i = threadIdx.x; i < slots; i += PREP_THREADS) {
+            const uint32_t owner = (uint32_t)((i / K) % ctas);
+            if ((int)owner == rank) continue;
+            uint16_t id;
+            asm volatile("ld.shared::cluster.u16 %0, [%1];"
+                         : "=h"(id)
+                         : "r"(sm100::mapa_shared(sm100::smem_u32(s_id + i), owner))
+                         : "memory");
+            s_id[i] = (short)id;
+        }
+        asm volatile("barrier.cluster.arrive.release;" ::: "memory");
     }
     __syncthreads();
     // rank of each choice among its expert's, in (token, choice) order: within 32 slots, then over those before
@@ -275,16 +404,13 @@ __global__ void __launch_bounds__(PREP_THREADS) moe_prep(const PrepParams p) {
         const uint32_t code = scale_code(m);
         uint32_t w0, w1, w2;
         quantize16(v, e8m0_reciprocal(code), nan, w0, w1, w2);
-        load_unit(u + gridDim.x * WARPS, v);
+        load_unit(p, u + gridDim.x * WARPS, units, chunks, vec, v);
         if (col >= p.hidden) continue;
 #pragma unroll 4
         for (int j = 0; j < K; j++) {
             const int row = s_id[t * K + j], place = s_place[t * K + j], r = place & 127;
             if (row < 0) continue;
-            *reinterpret_cast<uint4*>(p.xq + (size_t)row * p.hidden + col) = make_uint4(w0, w1, w2, 0u);
-            if ((lane & 1) == 0)
-                p.sx[((size_t)(place >> 7) * k_slabs + col / 128) * 512 + (r % 32) * 16 + (r / 32) * 4 + (col / 32) % 4] =
-                    (uint8_t)code;
+            store_unit(p, row, place >> 7, r, col, make_uint4(w0, w1, w2, 0u), code);
         }
     }
 }
@@ -391,10 +517,19 @@ __global__ void __launch_bounds__(ProductConfig<KIND, NMAX>::THREADS, ProductCon
     __syncthreads();
     sm100::tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    sm100::griddep_wait();
-    sm100::griddep_launch_dependents();
-
+    // The up product lets the down product start only after its own griddepcontrol.wait, that is once the list of
+    // entries, and whatever wrote the weights, is complete. So the down product reads the list, and loads its first weight
+    // tiles, while the up product still runs; its tokens (the hidden values) and outputs wait. Tokens go with the wait
+    // in warp 0, outputs in warps 2..5.
+    constexpr bool EARLY = KIND == KIND_DOWN;
+    if (!EARLY) sm100::griddep_wait();
+    // the first item's entry is read beside the count (it exists in the workspace whatever the count is)
+    const Entry first = p.entries[blockIdx.x / p.tiles];
     const int total = *p.n_entries * p.tiles;
+    if (EARLY && warp != 0) sm100::griddep_wait();
+    if (!EARLY || warp != 0) sm100::griddep_launch_dependents();
+    // the entry of item `it`, read an item ahead of its use
+    auto entry_at = [&](int it) { return it < total ? p.entries[it / p.tiles] : Entry{0, 0, 0, 0}; };
     uint32_t issued_mask = 0, issued_phase = 0;
     bool mma_issued = false;
 
@@ -403,27 +538,48 @@ __global__ void __launch_bounds__(ProductConfig<KIND, NMAX>::THREADS, ProductCon
             int stage = 0;
             uint32_t phase = 0;
             bool ok = true;
+            Entry next = first;
+            // Before the wait (EARLY): the weights of this many of the first item's slabs; their tokens follow it.
+            const int ahead = EARLY && (int)blockIdx.x < total ? min(C::STAGES, p.k_slabs) : 0;
+            auto load_weights = [&](int st, int row0, int kb) {
+                const uint32_t fb = full_bar(st), dst = base + st * C::STAGE;
+                sm100::tma_load_2d(dst, &tmW, fb, kb * 128, row0);
+                if (C::GATED) sm100::tma_load_2d(dst + 64 * 128, &tmW, fb, kb * 128, row0 + p.inter);
+                if (!C::GATED)
+                    sm100::bulk_load(sf_base + st * C::SF_BYTES, p.sW + ((size_t)(row0 / 128) * p.k_slabs + kb) * 512, 512, fb);
+            };
             for (int it = blockIdx.x; it < total && ok; it += gridDim.x) {
                 const int a = it / p.tiles, tile = it - a * p.tiles;
-                const Entry en = p.entries[a];
+                const Entry en = next;
+                next = entry_at(it + gridDim.x);
                 const int boxes = (en.n + 15) / 16;
                 const int row0 = en.expert * p.rows_per_expert + tile * (C::GATED ? 64 : 128);
                 const uint32_t tx = 128u * 96u + 2048u * boxes + (C::GATED ? 512u : 1024u);
-                for (int kb = 0; kb < p.k_slabs; kb++) {
-                    if (!sm100::wait_parity_bounded(empty_bar(stage), phase ^ 1u, abort_flag, p.wait_budget)) {
-                        raise(0x1u);
-                        ok = false;
-                        break;
+                const int done = it == (int)blockIdx.x ? ahead : 0;
+                if (EARLY && it == (int)blockIdx.x) {
+                    for (int kb = 0; kb < ahead; kb++) {  // the ring is empty: no wait
+                        sm100::mbar_arrive_expect_tx(full_bar(kb), tx);
+                        load_weights(kb, row0, kb);
+                        issued_mask |= 1u << kb;
                     }
-                    const uint32_t fb = full_bar(stage), a_dst = base + stage * C::STAGE;
-                    sm100::mbar_arrive_expect_tx(fb, tx);
-                    sm100::tma_load_2d(a_dst, &tmW, fb, kb * 128, row0);
-                    if (C::GATED) sm100::tma_load_2d(a_dst + 64 * 128, &tmW, fb, kb * 128, row0 + p.inter);
+                    sm100::griddep_wait();
+                    sm100::griddep_launch_dependents();
+                }
+                for (int kb = 0; kb < p.k_slabs; kb++) {
+                    const uint32_t fb = full_bar(stage);
+                    if (kb >= done) {
+                        if (!sm100::wait_parity_bounded(empty_bar(stage), phase ^ 1u, abort_flag, p.wait_budget)) {
+                            raise(0x1u);
+                            ok = false;
+                            break;
+                        }
+                        sm100::mbar_arrive_expect_tx(fb, tx);
+                        load_weights(stage, row0, kb);
+                    }
                     for (int b = 0; b < boxes; b++)
-                        sm100::tma_load_2d(a_dst + C::A_BYTES + 2048 * b, &tmB, fb, kb * 128, en.start + 16 * b);
-                    const uint32_t sf = sf_base + stage * C::SF_BYTES;
-                    if (!C::GATED) sm100::bulk_load(sf, p.sW + ((size_t)(row0 / 128) * p.k_slabs + kb) * 512, 512, fb);
-                    sm100::bulk_load(sf + 512, p.sB + ((size_t)a * p.k_slabs + kb) * 512, 512, fb);
+                        sm100::tma_load_2d(base + stage * C::STAGE + C::A_BYTES + 2048 * b, &tmB, fb, kb * 128,
+                                           en.start + 16 * b);
+                    sm100::bulk_load(sf_base + stage * C::SF_BYTES + 512, p.sB + ((size_t)a * p.k_slabs + kb) * 512, 512, fb);
                     issued_mask |= 1u << stage;
                     issued_phase = (issued_phase & ~(1u << stage)) | (phase << stage);
                     if (++stage == C::STAGES) {
@@ -433,13 +589,22 @@ __global__ void __launch_bounds__(ProductConfig<KIND, NMAX>::THREADS, ProductCon
                 }
             }
         }
+        // a down product without items still ends after the up product
+        if (EARLY && (lane != 0 || (int)blockIdx.x >= total)) {
+            sm100::griddep_wait();
+            sm100::griddep_launch_dependents();
+        }
     } else if (warp == 1) {
         if (lane == 0) {
             int stage = 0, local = 0;
             uint32_t phase = 0;
             bool ok = true;
+            Entry next = first;
+            // the next slab's barrier is polled right after a slab's MMAs are issued: the pipe's queue is short
+            bool ready = false;
             for (int it = blockIdx.x; it < total && ok; it += gridDim.x, local++) {
-                const int n = p.entries[it / p.tiles].n;
+                const int n = next.n;
+                next = entry_at(it + gridDim.x);
                 const uint32_t idesc = sm100::make_idesc_e2m3(128, (n + 15) / 16 * 16);
                 const int b = local & 1;
                 const uint32_t d_taddr = tmem_base + b * NMAX;
@@ -449,12 +614,11 @@ __global__ void __launch_bounds__(ProductConfig<KIND, NMAX>::THREADS, ProductCon
                 }
                 sm100::tc_fence_after();
                 for (int kb = 0; kb < p.k_slabs; kb++) {
-                    if (!sm100::wait_parity_bounded(full_bar(stage), phase, abort_flag, p.wait_budget)) {
+                    if (!ready && !sm100::wait_parity_bounded(full_bar(stage), phase, abort_flag, p.wait_budget)) {
                         raise(0x2u);
                         ok = false;
                         break;
                     }
-                    sm100::tc_fence_after();
                     const uint32_t sf = sf_base + stage * C::SF_BYTES;
                     sm100::tc_cp_32x128b_warpx4(tmem_base + C::TMEM_SFA, sm100::make_sf_desc(sf));
                     sm100::tc_cp_32x128b_warpx4(tmem_base + C::TMEM_SFB, sm100::make_sf_desc(sf + 512));
@@ -472,6 +636,7 @@ __global__ void __launch_bounds__(ProductConfig<KIND, NMAX>::THREADS, ProductCon
                         stage = 0;
                         phase ^= 1u;
                     }
+                    ready = sm100::mbar_test_wait(full_bar(stage), phase);
                 }
                 if (ok) sm100::tc_commit(acc_full0 + 8u * b);
             }
@@ -479,9 +644,11 @@ __global__ void __launch_bounds__(ProductConfig<KIND, NMAX>::THREADS, ProductCon
     } else if (warp < 6) {
         const int quarter = warp & 3;
         int local = 0;
+        Entry next = first;
         for (int it = blockIdx.x; it < total; it += gridDim.x, local++) {
             const int a = it / p.tiles, tile = it - a * p.tiles;
-            const Entry en = p.entries[a];
+            const Entry en = next;
+            next = entry_at(it + gridDim.x);
             const int b = local & 1;
             // all four warps leave together on a timeout (they share a barrier below)
             const bool got = sm100::wait_parity_bounded(acc_full0 + 8u * b, (local >> 1) & 1, abort_flag, p.wait_budget);
@@ -567,9 +734,11 @@ __global__ void __launch_bounds__(ProductConfig<KIND, NMAX>::THREADS, ProductCon
         int stage = 0;
         uint32_t phase = 0;
         bool ok = true;
+        Entry next = first;
         for (int it = blockIdx.x; it < total && ok; it += gridDim.x) {
             const int a = it / p.tiles, tile = it - a * p.tiles;
-            const int row0 = p.entries[a].expert * p.rows_per_expert + tile * 64;
+            const int row0 = next.expert * p.rows_per_expert + tile * 64;
+            next = entry_at(it + gridDim.x);
             const uint8_t* gate = p.sW + (size_t)(row0 / 128) * p.k_slabs * 512 + lane * 16 + (row0 % 128) / 32 * 4;
             const uint8_t* up = gate + (size_t)(p.inter / 128) * p.k_slabs * 512;
             for (int kb = 0; kb < p.k_slabs; kb++) {
@@ -637,20 +806,26 @@ struct CombineParams {
 // Four columns of one token per thread; hidden % 128 == 0.
 __global__ void __launch_bounds__(256) moe_combine(const CombineParams p) {
     sm100::griddep_launch_dependents();
+    // the places and weights were complete when the down product let this kernel start (see moe_product): read them
+    // before the wait
+    const int t = blockIdx.y, col = (blockIdx.x * blockDim.x + threadIdx.x) * 4, lane = threadIdx.x & 31;
+    const int slot = lane < p.top_k ? p.slot_of[t * p.top_k + lane] : -1;
+    const float weight = lane < p.top_k ? p.slot_w[t * p.top_k + lane] : 0.0f;
     sm100::griddep_wait();
-    const int t = blockIdx.y, col = (blockIdx.x * blockDim.x + threadIdx.x) * 4;
-    if (col >= p.hidden) return;
     float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    const bool in = col < p.hidden;
+#pragma unroll 4
     for (int j = 0; j < p.top_k; j++) {
-        const int s = p.slot_of[t * p.top_k + j];
-        if (s < 0) continue;
-        const float w = p.slot_w[t * p.top_k + j];
+        const int s = __shfl_sync(0xffffffffu, slot, j);
+        const float w = __shfl_sync(0xffffffffu, weight, j);
+        if (s < 0 || !in) continue;
         const float4 q = *reinterpret_cast<const float4*>(p.y + (size_t)s * p.hidden + col);
         v[0] += w * q.x;
         v[1] += w * q.y;
         v[2] += w * q.z;
         v[3] += w * q.w;
     }
+    if (!in) return;
     if (p.residual)
 #pragma unroll
         for (int i = 0; i < 4; i++) v[i] += kern::load_elem(p.residual, p.type, (size_t)t * p.ld_residual + col + i);
