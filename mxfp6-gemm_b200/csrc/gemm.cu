@@ -18,6 +18,7 @@
 #include <random>
 
 #include "gemm_kernel.cuh"
+#include "gemm_kernel_few.cuh"
 #include "gemm_kernel_pair.cuh"
 #include "host.hpp"
 #include "mxfp6/gemm.hpp"
@@ -688,6 +689,67 @@ bool launch_reduce_fused(const float* ws, const kern::Epi& epi, int M, int N, in
     return true;
 }
 
+template <int BN>
+bool launch_few(int S, int M, int N, int Kp, const void* dA, const void* dB, const uint8_t* sA, const uint8_t* sB,
+                int A_row_bytes, int B_row_bytes, cudaStream_t stream, const FusedLaunch& fused) {
+    using C = kern::FewConfig<BN>;
+    auto kernel = kern::gemm_mxfp6_few<BN>;
+    static std::once_flag attr_once[kMaxDevices];
+    static cudaError_t attr_err[kMaxDevices];
+    const int dev = current_device();
+    if (dev < 0 || dev >= kMaxDevices) {
+        set_error(MXFP6_ERR_CUDA, "no CUDA device");
+        return false;
+    }
+    const int rows = M <= 16 ? 16 : M <= 32 ? 32 : 64;
+    std::call_once(attr_once[dev], [&] {
+        int most = 0;
+        for (int r : {16, 32, 64})
+            if (C::smem_bytes(r) > most) most = C::smem_bytes(r);
+        attr_err[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    });
+    if (attr_err[dev] != cudaSuccess) {
+        set_error(MXFP6_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(attr_err[dev]));
+        return false;
+    }
+    CUtensorMap tmA, tmB;
+    if (!make_fp6_tmap(&tmA, dA, M, Kp, A_row_bytes, rows) || !make_fp6_tmap(&tmB, dB, fused.n_rows, Kp, B_row_bytes, BN)) {
+        set_error(MXFP6_ERR_CUDA, "cuTensorMapEncodeTiled failed for %dx%dx%d (status %d)", M, N, Kp, t_encode_status);
+        return false;
+    }
+    kern::FusedParams p = {};
+    p.epi = fused.epi;
+    p.sfA = sA;
+    p.sfB = sB;
+    p.M = M;
+    p.N = N;
+    p.Kp = Kp;
+    p.k_slabs = Kp / kern::BK;
+    p.splits = S;
+    p.wait_budget = wait_budget();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((N + BN - 1) / BN * S), 1, 1);
+    cfg.blockDim = dim3(kern::FEW_THREADS, 1, 1);
+    cfg.dynamicSmemBytes = C::smem_bytes(rows);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    set_pdl(attr[0]);
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)S;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = S > 1 ? 2 : 1;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, tmA, tmB, p, rows);
+    if (e == cudaSuccess) e = cudaGetLastError();
+    if (e != cudaSuccess) {
+        set_error(MXFP6_ERR_CUDA, "few-row GEMM launch failed: %s", cudaGetErrorString(e));
+        return false;
+    }
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+    return true;
+}
+
 // Columns of a fused launch's split-K partials: whole 32-column chunks.
 int partials_pitch(int N) {
     return (N + 31) / 32 * 32;
@@ -867,6 +929,16 @@ void gemm_entry(int ot, int M, int N, int Kp, const void* dA, const void* dB, co
 void run_validated(int ot, int M, int N, int Kp, const void* dA, const void* dB, const uint8_t* sA,
                    const uint8_t* sB, const kern::DstList& dl, int Ar, int Br, void* ws, size_t ws_bytes,
                    cudaStream_t stream, const FusedLaunch* fused) {
+    if (fused && a_mode(Kp, dA, Ar) == kern::A_TMA) {
+        const Route few = few_route(M, N, Kp, sm_count(), ot == MXFP6_OUT_F32 ? fp32_min_splits(Kp) : 1);
+        if (few.splits > 0) {
+            if (few.NT == 256)
+                launch_few<256>(few.splits, M, N, Kp, dA, dB, sA, sB, Ar, Br, stream, *fused);
+            else
+                launch_few<128>(few.splits, M, N, Kp, dA, dB, sA, sB, Ar, Br, stream, *fused);
+            return;
+        }
+    }
     Route r = route_for_out(ot, M, N, Kp);
     const int sms = sm_count();
     const int Nw = fused ? partials_pitch(N) : N;  // columns of the split-K partials

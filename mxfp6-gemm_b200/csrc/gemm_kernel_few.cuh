@@ -1,0 +1,276 @@
+#pragma once
+// The GEMM with a fused epilogue for few rows (M <= 64): one wave of CTAs, K split over a cluster.
+//
+// A cluster of S = 1..8 CTAs computes one 128 x BN tile, each over its own K segment, with the operand stages, scale
+// copies and MMAs of gemm_mxfp6_sm100 (gemm_kernel.cuh). Such a GEMM reads every weight once and is over in a few
+// microseconds, so what counts is the latency from the first load to the last store:
+//   * every SM gets weights to read (S is the largest that one wave of two CTAs per SM holds), and the K segments' sums meet in shared
+//     memory of the cluster instead of global memory and a second kernel: each CTA leaves its FP32 accumulator in its own
+//     shared memory (over the operand ring, which is idle by then) and, after a cluster barrier, sums a share of the
+//     tile's (row, 32 columns) groups over the S CTAs, in segment order;
+//   * the epilogue runs on those groups with a lane per column, spread over all warps of all CTAs. In the tensor-memory
+//     layout (a lane per row) 16 rows would leave every warp but one idle.
+// Rows past M come from whatever follows A's rows in shared memory (any bytes are valid codes) and end in accumulator
+// lanes nobody reads. Waits are bounded (gemm_kernel.cuh); after a timeout every thread still takes both cluster barriers.
+#include "gemm_kernel.cuh"
+
+namespace mxfp6 {
+namespace kern {
+
+constexpr int FEW_ROWS = 64;       // rows at most
+constexpr int FEW_CLUSTER = 8;     // K segments at most
+constexpr int FEW_THREADS = 256;
+// Rows a warp finishes together: one up to FEW_SINGLE rows, where there are more warps than groups of four, else four.
+constexpr int FEW_BATCH = 4, FEW_SINGLE = 16;
+
+template <int BN>
+struct FewConfig {
+    static constexpr int W_BYTES = BN * 128, SF_BYTES = 512 + BN / 128 * 512;
+    static constexpr int PITCH = BN + 4;  // floats between the rows of the accumulator in shared memory
+    static constexpr int TMEM_SFA = BN, TMEM_SFB = BN + 4, TMEM_COLS = BN == 256 ? 512 : 256;
+    static constexpr int BAR_BYTES = 256, MAX_STAGES = 12;
+    // A stages of `rows` (16, 32 or 64) rows. Two CTAs of the narrow tile share an SM: the next call's CTAs then set up, and
+    // wait for this one, beside it (1 x 4096 x 4096 back to back: 12.3 us with the whole SM, 7.5 us with half).
+    static constexpr int stage_bytes(int rows) { return rows * 128 + W_BYTES + SF_BYTES; }
+    static constexpr int stages(int rows) {
+        const int fit = ((BN == 256 ? 227 : 113) * 1024 - 1024 - BAR_BYTES) / stage_bytes(rows);
+        return fit < MAX_STAGES ? fit : MAX_STAGES;
+    }
+    static constexpr int smem_bytes(int rows) { return 1024 + stages(rows) * stage_bytes(rows) + BAR_BYTES; }
+    static_assert(8 * (2 * MAX_STAGES + 2) + 16 <= BAR_BYTES, "barrier area");
+    static_assert(stages(64) >= 3 && stages(64) * stage_bytes(64) >= FEW_ROWS * PITCH * 4, "the accumulator fits the ring");
+    static_assert(stages(16) * stage_bytes(16) >= 16 * PITCH * 4 && 16 * 128 + stages(16) * W_BYTES >= 128 * 128, "ring");
+};
+
+// R rows of 32 columns: lane l has the sums of column n. `in`: the column is inside D.
+template <int R>
+__device__ __forceinline__ void few_store(const Epi& e, int row0, int M, int n, bool in, float (&v)[R]) {
+    const int lane = threadIdx.x & 31;
+    if (e.bias && in) {
+        const float b = load_elem(e.bias, e.bias_type, (size_t)n);
+#pragma unroll
+        for (int i = 0; i < R; i++) v[i] += b;
+    }
+    float a[R];
+    if (e.aux_op != AUX_NONE) {
+#pragma unroll
+        for (int i = 0; i < R; i++)
+            a[i] = in && row0 + i < M ? load_elem(e.aux, e.aux_type, (size_t)(row0 + i) * (size_t)e.ld_aux + (size_t)n) : 0.0f;
+    }
+    activate_all<R>(e.act, v);
+    if (e.aux_op != AUX_NONE) {
+#pragma unroll
+        for (int i = 0; i < R; i++) epi_join(e.aux_op, v[i], a[i]);
+    }
+    if (e.out_type != T_MXFP6) {
+#pragma unroll
+        for (int i = 0; i < R; i++)
+            if (in && row0 + i < M) store_elem(e.out, e.out_type, (size_t)(row0 + i) * (size_t)e.ldd + (size_t)n, v[i]);
+        return;
+    }
+    // MXFP6: a row's 32 columns are one block. Magnitudes order like their bits (NaN does not count); four lanes' codes
+    // make 24 bits, and six lanes write the block's 24 bytes.
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+        if (row0 + i >= M) break;
+        const uint32_t mag = v[i] != v[i] ? 0u : __float_as_uint(fabsf(v[i]));
+        const uint32_t code = scale_code(__uint_as_float(__reduce_max_sync(0xffffffffu, mag)));
+        const uint32_t c = to_e2m3x2(0.0f, v[i] * e8m0_reciprocal(code)) & 0x3Fu;
+        const uint32_t c12 = c | (__shfl_down_sync(0xffffffffu, c, 1) << 6);
+        const uint32_t c24 = c12 | (__shfl_down_sync(0xffffffffu, c12, 2) << 12);  // 24 bits in every fourth lane
+        const int first = lane * 4 / 3;                                            // group in which word `lane` starts
+        const uint32_t lo = __shfl_sync(0xffffffffu, c24, 4 * first), hi = __shfl_sync(0xffffffffu, c24, 4 * first + 4);
+        const uint32_t w = lane % 3 == 0 ? lo | (hi << 24) : lane % 3 == 1 ? (lo >> 8) | (hi << 16) : (lo >> 16) | (hi << 8);
+        uint8_t* d = static_cast<uint8_t*>(e.out) + (size_t)(row0 + i) * (size_t)e.ldd + (size_t)((n - lane) / 4 * 3);
+        if (lane < 6) reinterpret_cast<uint32_t*>(d)[lane] = w;
+        if (lane == 6) e.scales[scale_atom_offset(row0 + i, (n - lane) / 32, e.k_atoms)] = (uint8_t)code;
+    }
+}
+
+// This CTA's share of the tile: tasks of 32 columns of R rows, summed over the cluster's accumulators at `here` in segment
+// order. All of a task's loads are in flight together.
+template <int BN, int R>
+__device__ __forceinline__ void few_finish(const FusedParams& p, int tile, int rank, int S, uint32_t here) {
+    using C = FewConfig<BN>;
+    constexpr int G = BN / 32;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint32_t part[FEW_CLUSTER];
+#pragma unroll
+    for (int s = 0; s < FEW_CLUSTER; s++) part[s] = s < S ? sm100::mapa_shared(here, (uint32_t)s) : 0u;
+    const int tasks = (p.M + R - 1) / R * G;
+    for (int t = rank + S * warp; t < tasks; t += S * (FEW_THREADS / 32)) {
+        const int row0 = t / G * R, c = t % G * 32 + lane, n = tile * BN + c;
+        if (n - lane >= p.N) continue;
+        const uint32_t at = (uint32_t)(row0 * C::PITCH + c) * 4u;
+        float q[FEW_CLUSTER][R], v[R];
+#pragma unroll
+        for (int s = 0; s < FEW_CLUSTER; s++)
+#pragma unroll
+            for (int i = 0; i < R; i++)
+                q[s][i] = s < S && row0 + i < p.M ? sm100::ld_cluster_f32(part[s] + at + (uint32_t)(i * C::PITCH * 4)) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+            v[i] = q[0][i];
+#pragma unroll
+            for (int s = 1; s < FEW_CLUSTER; s++)
+                if (s < S) v[i] += q[s][i];
+        }
+        few_store<R>(p.epi, row0, p.M, n, n < p.N, v);
+    }
+}
+
+// `rows`: A's rows in a stage (the tensor map's box). The cluster's rank is the K segment.
+template <int BN>
+__global__ void __launch_bounds__(FEW_THREADS, 1)
+    gemm_mxfp6_few(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const FusedParams p,
+                   const int rows) {
+    using C = FewConfig<BN>;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    const uint32_t raw_u32 = sm100::smem_u32(smem_raw);
+    const uint32_t base = (raw_u32 + 1023u) & ~1023u;
+    uint8_t* base_ptr = smem_raw + (base - raw_u32);
+    const int stages = C::stages(rows), x_bytes = rows * 128;
+    const uint32_t w_base = base + stages * x_bytes, sf_base = w_base + stages * C::W_BYTES;
+    const uint32_t bar_base = base + stages * C::stage_bytes(rows);
+    uint8_t* bar_ptr = base_ptr + stages * C::stage_bytes(rows);
+    auto full_bar = [&](int s) { return bar_base + 8u * s; };
+    auto empty_bar = [&](int s) { return bar_base + 8u * (C::MAX_STAGES + s); };
+    const uint32_t acc_full = bar_base + 8u * (2 * C::MAX_STAGES);
+    const uint32_t drain_bar = acc_full + 8u;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_ptr + 8 * (2 * C::MAX_STAGES + 2));
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(bar_ptr + 8 * (2 * C::MAX_STAGES + 2) + 8);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int S = (int)sm100::cluster_nctarank(), rank = (int)sm100::cluster_ctarank();
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < stages; s++) {
+            sm100::mbar_init(full_bar(s), 1);
+            sm100::mbar_init(empty_bar(s), 1);
+        }
+        sm100::mbar_init(acc_full, 1);
+        sm100::mbar_init(drain_bar, 1);
+        *abort_flag = 0;
+        sm100::fence_mbar_init();
+        sm100::fence_async_shared();
+        sm100::prefetch_tmap(&tmA);
+        sm100::prefetch_tmap(&tmB);
+    }
+    if (warp == 1) {
+        sm100::tmem_alloc(sm100::smem_u32(tmem_slot), C::TMEM_COLS);
+        sm100::tmem_relinquish();
+    }
+    sm100::tc_fence_before();
+    __syncthreads();
+    sm100::tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    sm100::griddep_launch_dependents();
+    sm100::griddep_wait();
+
+    const int tile = (int)blockIdx.x / S;
+    const int kb0 = (int)((long long)p.k_slabs * rank / S), kb1 = (int)((long long)p.k_slabs * (rank + 1) / S);
+    const int atoms = min(BN / 128, (p.N - tile * BN + 127) / 128);  // B's scale atoms inside the matrix
+    bool loads_issued = false, mma_issued = false;
+    if (warp == 0 && lane == 0) {
+        int stage = 0;
+        uint32_t phase = 0;
+        const uint32_t tx = (uint32_t)(rows * 96 + BN * 96 + 512 * (1 + atoms));
+        for (int kb = kb0; kb < kb1; kb++) {
+            if (!sm100::wait_parity_bounded(empty_bar(stage), phase ^ 1u, abort_flag, p.wait_budget)) {
+                if (!*abort_flag) raise_status(0x1u, abort_flag);
+                break;
+            }
+            const uint32_t fb = full_bar(stage), sf = sf_base + stage * C::SF_BYTES;
+            sm100::mbar_arrive_expect_tx(fb, tx);
+            sm100::tma_load_2d(w_base + stage * C::W_BYTES, &tmB, fb, kb * BK, tile * BN);
+            for (int j = 0; j < atoms; j++)
+                sm100::bulk_load(sf + 512 + 512 * j, p.sfB + ((size_t)(tile * (BN / 128) + j) * p.k_slabs + kb) * 512, 512, fb);
+            sm100::tma_load_2d(base + stage * x_bytes, &tmA, fb, kb * BK, 0);
+            sm100::bulk_load(sf, p.sfA + (size_t)kb * 512, 512, fb);
+            loads_issued = true;
+            if (++stage == stages) {
+                stage = 0;
+                phase ^= 1u;
+            }
+        }
+    } else if (warp == 1 && lane == 0) {
+        constexpr uint32_t idesc = sm100::make_idesc_e2m3(BM, BN);
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int kb = kb0; kb < kb1; kb++) {
+            if (!sm100::wait_parity_bounded(full_bar(stage), phase, abort_flag, p.wait_budget)) {
+                if (!*abort_flag) raise_status(0x2u, abort_flag);
+                ok = false;
+                break;
+            }
+            const uint32_t sf = sf_base + stage * C::SF_BYTES;
+            sm100::tc_cp_32x128b_warpx4(tmem_base + C::TMEM_SFA, sm100::make_sf_desc(sf));
+#pragma unroll
+            for (int j = 0; j < BN / 128; j++)
+                sm100::tc_cp_32x128b_warpx4(tmem_base + C::TMEM_SFB + 4 * j, sm100::make_sf_desc(sf + 512 + 512 * j));
+            const uint32_t a_src = base + stage * x_bytes, b_src = w_base + stage * C::W_BYTES;
+#pragma unroll
+            for (int k = 0; k < BK / 32; k++) {
+                const uint32_t sel = (uint32_t)k << 30;
+                sm100::tc_mma_mxf8f6f4(tmem_base, sm100::make_kmajor_sw128_desc(a_src + 32 * k),
+                                       sm100::make_kmajor_sw128_desc(b_src + 32 * k), sm100::idesc_with_sf_ids(idesc, k, k),
+                                       (tmem_base + C::TMEM_SFA) | sel, (tmem_base + C::TMEM_SFB) | sel,
+                                       kb > kb0 || k > 0 ? 1u : 0u);
+            }
+            mma_issued = true;
+            sm100::tc_commit(empty_bar(stage));
+            if (++stage == stages) {
+                stage = 0;
+                phase ^= 1u;
+            }
+        }
+        if (ok) sm100::tc_commit(acc_full);
+    }
+    __syncwarp();
+    // The accumulator to shared memory: a lane per row, half of the columns per warp.
+    const bool got = sm100::wait_parity_bounded(acc_full, 0, abort_flag, p.wait_budget);
+    if (!got && !*abort_flag) raise_status(0x4u, abort_flag);
+    const int aborted = __syncthreads_or(!got);
+    float* acc = reinterpret_cast<float*>(base_ptr);
+    if (!aborted) {
+        sm100::tc_fence_after();
+        const int quarter = warp & 3, row = 32 * quarter + lane;
+        if (32 * quarter < p.M) {
+#pragma unroll 1
+            for (int c = (warp >> 2) * (BN / 2); c < (warp >> 2) * (BN / 2) + BN / 2; c += 32) {
+                uint32_t r[32];
+                sm100::tmem_ld_32x32b_x32(tmem_base + ((uint32_t)(32 * quarter) << 16) + (uint32_t)c, r);
+                sm100::tmem_ld_wait(r);
+                if (row < p.M) {
+                    uint4* d = reinterpret_cast<uint4*>(acc + row * C::PITCH + c);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) d[i] = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
+                }
+            }
+        }
+        sm100::tc_fence_before();
+    } else {
+        // the other CTAs read whatever is here: let loads in flight land, and the MMAs finish, first
+        const int zero = 0;
+        if (loads_issued) sm100::settle_ns(200000);
+        if (mma_issued) {
+            sm100::tc_commit(drain_bar);
+            if (!sm100::wait_parity_bounded(drain_bar, 0, &zero, WAIT_BUDGET / 4)) atomicOr(&g_device_status, 0x8u);
+        }
+        sm100::tc_fence_before();
+    }
+    __syncthreads();
+    if (warp == 1) {
+        sm100::tc_fence_after();
+        sm100::tmem_dealloc(tmem_base, C::TMEM_COLS);
+    }
+    if (S > 1) sm100::cluster_sync();
+    if (p.M <= FEW_SINGLE)
+        few_finish<BN, 1>(p, tile, rank, S, sm100::smem_u32(acc));
+    else
+        few_finish<BN, FEW_BATCH>(p, tile, rank, S, sm100::smem_u32(acc));
+    if (S > 1) sm100::cluster_sync();  // no CTA leaves while another may read its accumulator
+}
+
+}  // namespace kern
+}  // namespace mxfp6

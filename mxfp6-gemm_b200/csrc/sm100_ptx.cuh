@@ -368,6 +368,13 @@ __device__ __forceinline__ uint32_t cluster_ctarank() {
     return r;
 }
 
+// One float of a CTA of the cluster's shared memory (shared::cluster address).
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+
 // CTAs in this cluster (1 for a launch without clusters).
 __device__ __forceinline__ uint32_t cluster_nctarank() {
     uint32_t r;
