@@ -34,23 +34,36 @@ struct Epi {
     int k_atoms;                     // MXFP6: N / 128
 };
 
-// Logistic sigmoid times v: v / (1 + e^-x). The quotient has no cancellation anywhere, and the
-// hardware exponential and division keep it within a few FP32 ulp.
+// 2^x and 1/x by the hardware approximations (2 and 1 ulp), which flush subnormal results to 0: without .ftz each carries
+// instructions that rescale its argument.
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+constexpr float LOG2E = 1.4426950408889634f;
+
+// Logistic sigmoid times v: v / (1 + e^-x). The quotient has no cancellation anywhere, so it stays within a few FP32 ulp.
 __device__ __forceinline__ float times_sigmoid(float v, float x) {
-    return __fdividef(v, 1.0f + __expf(-x));
+    return v * rcp(1.0f + ex2(-LOG2E * x));
 }
 
 // v Phi(v) = v (1 - erfc(v / sqrt(2)) / 2) for v >= 0 and v erfc(-v / sqrt(2)) / 2 below, with
 // erfc(x) = (a1 t + ... + a5 t^5) e^(-x^2), t = 1 / (1 + p x) for x >= 0 (Hastings; Abramowitz and Stegun
-// 7.1.26: absolute error 1.5e-7). It has no branch, so a chunk's 32 evaluations overlap.
+// 7.1.26: absolute error 1.5e-7; the coefficients here are halved, and e^(-x^2) = 2^(-v^2 log2(e) / 2)). It has no
+// branch, so a chunk's evaluations overlap.
 __device__ __forceinline__ float gelu_erf(float v) {
-    const float x = fabsf(v) * 0.70710678118654752f;
-    const float t = __fdividef(1.0f, fmaf(0.3275911f, x, 1.0f));
-    float q = fmaf(1.061405429f, t, -1.453152027f);
-    q = fmaf(q, t, 1.421413741f);
-    q = fmaf(q, t, -0.284496736f);
-    q = fmaf(q, t, 0.254829592f);
-    const float half_erfc = 0.5f * q * t * __expf(-x * x);
+    const float t = rcp(fmaf(0.3275911f * 0.70710678118654752f, fabsf(v), 1.0f));
+    float q = fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
+    q = fmaf(q, t, 0.5f * 1.421413741f);
+    q = fmaf(q, t, 0.5f * -0.284496736f);
+    q = fmaf(q, t, 0.5f * 0.254829592f);
+    const float half_erfc = q * t * ex2(-0.5f * LOG2E * v * v);
     return v * (v < 0.0f ? half_erfc : 1.0f - half_erfc);
 }
 
