@@ -229,12 +229,42 @@ __device__ __forceinline__ void store_words(void* dst, const uint32_t* w, bool a
     }
 }
 
-// One lane's aux operand of a chunk as loaded (FP32: 32 words, else 16). It is loaded a chunk ahead of
-// its use: the loads of the next chunk are in flight while this one is computed and stored.
-struct AuxRaw {
+// One lane's aux operand of a chunk as loaded. It is loaded a chunk ahead of its use: the loads of the next chunk are in
+// flight while this one is computed and stored. Row layout (lane = row): 32 columns (FP32: 32 words, else 16). Column
+// layout (lane = column): a word for each of 32 rows, 16-bit elements in its low half.
+template <bool COLUMNS>
+struct AuxRaw;
+template <>
+struct AuxRaw<false> {
     uint4 q[8];
 };
-__device__ __forceinline__ void epi_load_aux(const Epi& e, int row, int col, bool live, AuxRaw& a) {
+template <>
+struct AuxRaw<true> {
+    uint32_t w[32];
+};
+__device__ __forceinline__ void epi_load_aux(const Epi& e, int row0, int M, int col, int N, AuxRaw<true>& a) {
+    const int c = col + (threadIdx.x & 31), rows = M - row0;
+    if (e.aux_op == AUX_NONE || rows <= 0 || col < 0 || c >= N) return;
+    const size_t i = (size_t)row0 * (size_t)e.ld_aux + (size_t)c;
+    if (e.aux_type == T_F32) {
+        const uint32_t* s = static_cast<const uint32_t*>(e.aux) + i;
+#pragma unroll
+        for (int k = 0; k < 32; k++) {
+            if (k < rows) a.w[k] = *s;
+            s += e.ld_aux;
+        }
+    } else {
+        const uint16_t* s = static_cast<const uint16_t*>(e.aux) + i;
+#pragma unroll
+        for (int k = 0; k < 32; k++) {
+            if (k < rows) a.w[k] = *s;
+            s += e.ld_aux;
+        }
+    }
+}
+__device__ __forceinline__ void epi_load_aux(const Epi& e, int row0, int M, int col, int N, AuxRaw<false>& a) {
+    const int row = row0 + (threadIdx.x & 31);
+    const bool live = row < M && col >= 0 && col + 32 <= N;
     if (e.aux_op == AUX_NONE || !e.aux_vec || !live) return;
     const size_t i = (size_t)row * (size_t)e.ld_aux + (size_t)col;
     const uint4* s = e.aux_type == T_F32 ? reinterpret_cast<const uint4*>(static_cast<const float*>(e.aux) + i)
@@ -256,7 +286,7 @@ __device__ __forceinline__ void epi_join(int op, float& v, float a) {
 constexpr int EPI_TILE_PITCH = 36;
 constexpr int EPI_TILE_BYTES = 32 * EPI_TILE_PITCH * 4;
 
-// The warp's rows of a chunk from its shared-memory tile, lane = column, eight rows at a time.
+// The warp's rows of the last, partial chunk from its shared-memory tile, lane = column, eight rows at a time.
 // `in`: the lane's column is inside D.
 template <int OT>
 __device__ __forceinline__ void epi_rows(const Epi& e, int row0, int rows, int col, bool in, float bias,
@@ -299,18 +329,85 @@ __device__ __forceinline__ void epi_rows(const Epi& e, int row0, int rows, int c
     }
 }
 
-// The epilogue of a warp's chunk: lane l holds the accumulators of columns [col, col + 32) of row
-// row0 + l. `valid` = N - col (> 0, the same in every lane), `aux` the lane's aux operand when
-// e.aux_vec is set and the chunk is whole, `bias` the chunk's 32 values in shared memory (zeros
-// without a bias), `tile` this warp's.
-//
-// Whole chunks of aligned outputs stay in this layout. Others (odd N, odd pitch, the last columns)
-// go through `tile` to lane = column, so that a store instruction covers consecutive addresses of one
-// row: a per-lane row would touch 32 sectors with each 4-byte store.
+// bias and activation of a lane's row of a chunk, `bias` the chunk's 32 values in shared memory (zeros without a bias).
+__device__ __forceinline__ void epi_activate(const Epi& e, const uint32_t (&r)[32], const float* bias, float (&v)[32]) {
+#pragma unroll
+    for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
+    if (e.bias) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float4 q = reinterpret_cast<const float4*>(bias)[i];
+            v[4 * i] += q.x;
+            v[4 * i + 1] += q.y;
+            v[4 * i + 2] += q.z;
+            v[4 * i + 3] += q.w;
+        }
+    }
+    activate_all<32>(e.act, v);
+}
+
+// The warp's activated rows from its shared-memory tile, lane = column: aux, and a store of consecutive addresses of one
+// row at a time. AT: aux type, or -1 for none.
+template <int OT, int AT>
+__device__ __forceinline__ void epi_columns(const Epi& e, int row0, int rows, int col, bool in, const AuxRaw<true>& a,
+                                            const float* tile) {
+    using Out = std::conditional_t<OT == T_F32, float, std::conditional_t<OT == T_F16, __half, __nv_bfloat16>>;
+    Out* out = static_cast<Out*>(e.out) + (size_t)row0 * (size_t)e.ldd + (size_t)col;
+#pragma unroll
+    for (int k = 0; k < 32; k++) {
+        float v = tile[k * EPI_TILE_PITCH];
+        if constexpr (AT >= 0) {
+            uint32_t w = a.w[k];
+            asm volatile("" : "+r"(w));  // convert here: hoisted to the load, the conversion would wait for it
+            epi_join(e.aux_op, v, AT == T_F32 ? __uint_as_float(w)
+                                  : AT == T_F16 ? __half2float(__ushort_as_half((unsigned short)w)) : __uint_as_float(w << 16));
+        }
+        if (in && k < rows) store_elem(out, OT, 0, v);
+        out += e.ldd;
+    }
+}
+template <int OT>
+__device__ __forceinline__ void epi_columns(const Epi& e, int row0, int rows, int col, bool in, const AuxRaw<true>& a,
+                                            const float* tile) {
+    if (e.aux_op == AUX_NONE)
+        epi_columns<OT, -1>(e, row0, rows, col, in, a, tile);
+    else if (e.aux_type == T_F32)
+        epi_columns<OT, T_F32>(e, row0, rows, col, in, a, tile);
+    else if (e.aux_type == T_F16)
+        epi_columns<OT, T_F16>(e, row0, rows, col, in, a, tile);
+    else
+        epi_columns<OT, T_BF16>(e, row0, rows, col, in, a, tile);
+}
+
+// The epilogue of a warp's chunk, in the column layout: for outputs whose rows are not 16-byte aligned (odd N, odd pitch),
+// or whose aux operand's are not. Lane l holds the accumulators of columns [col, col + 32) of row row0 + l; after the
+// activation the chunk goes through `tile`, this warp's shared-memory tile, to lane = column, because a lane per row would
+// touch 32 sectors with each 2- or 4-byte access. `valid` = N - col (> 0, the same in every lane).
 __device__ __forceinline__ void epi_chunk(const Epi& e, int row0, int M, int col, int valid, const uint32_t (&r)[32],
-                                          const AuxRaw& aux, const float* bias, float* tile) {
+                                          const AuxRaw<true>& aux, const float* bias, float* tile) {
+    const int lane = threadIdx.x & 31, rows = M - row0;
+    if (rows <= 0) return;
+    float v[32];
+    epi_activate(e, r, bias, v);
+    float4* mine = reinterpret_cast<float4*>(tile + lane * EPI_TILE_PITCH);
+#pragma unroll
+    for (int i = 0; i < 8; i++) mine[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    __syncwarp();
+    if (e.out_type == T_F32)
+        epi_columns<T_F32>(e, row0, rows, col + lane, lane < valid, aux, tile + lane);
+    else if (e.out_type == T_F16)
+        epi_columns<T_F16>(e, row0, rows, col + lane, lane < valid, aux, tile + lane);
+    else
+        epi_columns<T_BF16>(e, row0, rows, col + lane, lane < valid, aux, tile + lane);
+    __syncwarp();  // the tile is rewritten by the next chunk
+}
+
+// The same in the row layout: every lane stores its row's 32 columns with wide accesses, and of an MXFP6 output
+// quantises them, since they are one block. The last chunk of a width that is no multiple of 32 goes through `tile`.
+__device__ __forceinline__ void epi_chunk(const Epi& e, int row0, int M, int col, int valid, const uint32_t (&r)[32],
+                                          const AuxRaw<false>& aux, const float* bias, float* tile) {
     const int lane = threadIdx.x & 31, row = row0 + lane;
-    if (e.out_type != T_MXFP6 && (!e.out_vec || valid < 32)) {
+    if (e.out_type != T_MXFP6 && valid < 32) {
         const int rows = M - row0 < 32 ? M - row0 : 32;
         if (rows <= 0) return;
         uint4* mine = reinterpret_cast<uint4*>(tile + lane * EPI_TILE_PITCH);
@@ -329,19 +426,7 @@ __device__ __forceinline__ void epi_chunk(const Epi& e, int row0, int M, int col
     }
     if (row >= M) return;
     float v[32];
-#pragma unroll
-    for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
-    if (e.bias) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const float4 q = reinterpret_cast<const float4*>(bias)[i];
-            v[4 * i] += q.x;
-            v[4 * i + 1] += q.y;
-            v[4 * i + 2] += q.z;
-            v[4 * i + 3] += q.w;
-        }
-    }
-    activate_all<32>(e.act, v);
+    epi_activate(e, r, bias, v);
     if (e.aux_op != AUX_NONE) {
         if (!e.aux_vec) {  // MXFP6 output only
 #pragma unroll

@@ -464,7 +464,7 @@ template <typename OutT, bool PARTIAL>
 int out_align32(const float* ws, const kern::DstList& dl) {
     if constexpr (PARTIAL)
         return aligned(ws, 32) ? 1 : 0;
-    else if constexpr (std::is_same<OutT, kern::FusedOut>::value)
+    else if constexpr (kern::FusedTraits<OutT>::fused)
         return 0;  // the fused epilogue keeps its own alignment flags
     else
         return dst_align32(dl, sizeof(OutT)) ? 1 : 0;
@@ -476,7 +476,7 @@ bool launch_gemm(int M, int N, int Kp, const void* dA, const void* dB, const uin
                  int splits, cudaStream_t stream, const FusedLaunch* fused = nullptr) {
     using C = kern::Config<BN, AMODE>;
     auto kernel = kern::gemm_mxfp6_sm100<BN, OutT, PARTIAL, AMODE>;
-    constexpr int smem_bytes = std::is_same<OutT, kern::FusedOut>::value ? C::FUSED_SMEM_BYTES : C::SMEM_BYTES;
+    constexpr int smem_bytes = kern::FusedTraits<OutT>::fused ? C::FUSED_SMEM_BYTES : C::SMEM_BYTES;
     static std::once_flag attr_once[kMaxDevices];
     const int dev = current_device();
     if (dev < 0 || dev >= kMaxDevices) {
@@ -499,7 +499,7 @@ bool launch_gemm(int M, int N, int Kp, const void* dA, const void* dB, const uin
         return false;
     }
     kern::ParamsFor<OutT> p;
-    if constexpr (std::is_same<OutT, kern::FusedOut>::value) p.epi = fused->epi;
+    if constexpr (kern::FusedTraits<OutT>::fused) p.epi = fused->epi;
     p.sfA = sA;
     p.sfB = sB;
     p.dst = dl;
@@ -550,7 +550,7 @@ bool launch_pair(int M, int N, int Kp, const void* dA, const void* dB, const uin
     // both (one instantiation in partial mode, which has neither)
     auto kernel_lean = kern::gemm_mxfp6_sm100_pair<OutT, PARTIAL, AMODE, kern::EPI_LEAN>;
     auto kernel_sk = kern::gemm_mxfp6_sm100_pair<OutT, PARTIAL, AMODE, PARTIAL ? kern::EPI_LEAN : kern::EPI_STREAM_K>;
-    constexpr bool FUSED = std::is_same<OutT, kern::FusedOut>::value;  // one destination, always
+    constexpr bool FUSED = kern::FusedTraits<OutT>::fused;  // one destination, always
     constexpr int smem_bytes = FUSED ? C::FUSED_SMEM_BYTES : C::SMEM_BYTES;
     auto kernel_all = kern::gemm_mxfp6_sm100_pair<OutT, PARTIAL, AMODE,
                                                   PARTIAL ? kern::EPI_LEAN : FUSED ? kern::EPI_STREAM_K : kern::EPI_ALL>;
@@ -789,7 +789,7 @@ bool run_route(const Route& r, int M, int N, int Kp, const void* dA, const void*
                   : launch_gemm<128, OutT, false, AMODE>(M, N, Kp, dA, dB, sA, sB, dl, wsf, Ar, Br, 1, stream, fused);
     }
     if (!ok || !part) return ok;
-    if constexpr (std::is_same<OutT, kern::FusedOut>::value)
+    if constexpr (kern::FusedTraits<OutT>::fused)
         return launch_reduce_fused(wsf, fused->epi, M, n_real, N, r.splits, stream);
     else
         return launch_reduce<OutT>(wsf, dl, M, N, r.splits, stream);
@@ -806,11 +806,19 @@ bool run_typed(const Route& r, int M, int N, int Kp, const void* dA, const void*
 bool run(int ot, const Route& r, int M, int N, int Kp, const void* dA, const void* dB, const uint8_t* sA,
          const uint8_t* sB, const kern::DstList& dl, int Ar, int Br, void* ws, cudaStream_t stream,
          const FusedLaunch* fused = nullptr) {
-    if (fused)
-        return a_mode(Kp, dA, Ar) == kern::A_TMA
-                   ? run_route<kern::FusedOut, kern::A_TMA>(r, M, N, Kp, dA, dB, sA, sB, dl, Ar, Br, ws, stream, fused)
-                   : run_route<kern::FusedOut, kern::A_CPASYNC>(r, M, N, Kp, dA, dB, sA, sB, dl, Ar, Br, ws, stream,
-                                                                fused);
+    if (fused) {
+        const bool tma = a_mode(Kp, dA, Ar) == kern::A_TMA;
+        // the column layout for unaligned rows, and for an FP32 aux operand of an FP32 output, whose loads a lane per
+        // row would spread over 32 lines each (3000 x 3104 x 512, FP32 with residual: 25.9 us by rows, 18.9 by columns)
+        const kern::Epi& e = fused->epi;
+        if (e.out_type != kern::T_MXFP6 &&
+            (!e.out_vec || (e.out_type == kern::T_F32 && e.aux_op != kern::AUX_NONE && e.aux_type == kern::T_F32)))
+            return tma ? run_route<kern::Fused<true>, kern::A_TMA>(r, M, N, Kp, dA, dB, sA, sB, dl, Ar, Br, ws, stream, fused)
+                       : run_route<kern::Fused<true>, kern::A_CPASYNC>(r, M, N, Kp, dA, dB, sA, sB, dl, Ar, Br, ws, stream,
+                                                                       fused);
+        return tma ? run_route<kern::FusedOut, kern::A_TMA>(r, M, N, Kp, dA, dB, sA, sB, dl, Ar, Br, ws, stream, fused)
+                   : run_route<kern::FusedOut, kern::A_CPASYNC>(r, M, N, Kp, dA, dB, sA, sB, dl, Ar, Br, ws, stream, fused);
+    }
     switch (ot) {
         case MXFP6_OUT_F32:
             return run_typed<float>(r, M, N, Kp, dA, dB, sA, sB, dl, Ar, Br, ws, stream);

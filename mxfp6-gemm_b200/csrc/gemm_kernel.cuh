@@ -117,15 +117,26 @@ struct Params {
     int band_L, band_a, band_n;
 };
 
-// Output type tag of the launches with a fused epilogue (epilogue.cuh), whose parameters carry it;
+// Output type tags of the launches with a fused epilogue (epilogue.cuh), whose parameters carry it;
 // D, its element type and its pitch are then in `epi`, and `dst` is unused. M and N may have any
-// positive value there: the tensor loads read zeros past the operands' last rows.
-struct FusedOut {};
+// positive value there: the tensor loads read zeros past the operands' last rows. COLUMNS: the column layout, for rows
+// without 16-byte alignment.
+template <bool COLUMNS>
+struct Fused {};
+using FusedOut = Fused<false>;
+template <typename T>
+struct FusedTraits {
+    static constexpr bool fused = false, columns = false;
+};
+template <bool COLUMNS>
+struct FusedTraits<Fused<COLUMNS>> {
+    static constexpr bool fused = true, columns = COLUMNS;
+};
 struct FusedParams : Params {
     Epi epi;
 };
 template <typename OutT>
-using ParamsFor = std::conditional_t<std::is_same<OutT, FusedOut>::value, FusedParams, Params>;
+using ParamsFor = std::conditional_t<FusedTraits<OutT>::fused, FusedParams, Params>;
 
 struct TileCoord {
     int mb, nb, split, kb_begin, kb_count;
@@ -228,7 +239,7 @@ __device__ __forceinline__ void store_rows_regrouped(const DstList& dl, uint8_t*
     __syncwarp();  // the staging area is rewritten by the next group
 }
 
-// OutT: float / __half / __nv_bfloat16, or FusedOut. PARTIAL: write FP32 partial sums to p.ws instead of D.
+// OutT: float / __half / __nv_bfloat16, or Fused. PARTIAL: write FP32 partial sums to p.ws instead of D.
 // AMODE (compact_a.cuh): A_TMA loads A with the 16U6 tensor load; A_CPASYNC adds four
 // loader warps that copy the A image from p.a_ptr (tmA unused).
 template <int BN, typename OutT, bool PARTIAL, int AMODE = A_TMA>
@@ -237,7 +248,7 @@ __global__ void __launch_bounds__(threads_for(AMODE), 1)
                      const ParamsFor<OutT> p) {
     using C = Config<BN, AMODE>;
     constexpr bool COMPACT = AMODE != A_TMA;
-    constexpr bool FUSED = std::is_same<OutT, FusedOut>::value;
+    constexpr bool FUSED = FusedTraits<OutT>::fused;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     // 1024-byte alignment for the 128-byte-swizzled operand tiles.
     const uint32_t raw_u32 = sm100::smem_u32(smem_raw);
@@ -426,10 +437,10 @@ __global__ void __launch_bounds__(threads_for(AMODE), 1)
             const TileCoord tc = decode_tile(t, p);
             const int row = tc.mb * BM + 32 * quarter + lane;
             const int col0 = tc.nb * BN;
-            [[maybe_unused]] AuxRaw aux[2];
+            [[maybe_unused]] AuxRaw<FusedTraits<OutT>::columns> aux[2];
             [[maybe_unused]] float* tile = reinterpret_cast<float*>(bar_ptr + C::BAR_BYTES + quarter * (EPI_TILE_BYTES + BN * 4));
             if constexpr (FUSED) {
-                epi_load_aux(p.epi, row, col0, row < p.M && col0 + 32 <= p.N, aux[0]);
+                epi_load_aux(p.epi, row - lane, p.M, col0, p.N, aux[0]);
                 epi_load_bias<BN / 32>(p.epi, col0, 32, p.N, tile + EPI_TILE_BYTES / 4);
             }
             if (!sm100::wait_parity_bounded(acc_full, acc_phase, abort_flag, p.wait_budget)) {
@@ -445,7 +456,7 @@ __global__ void __launch_bounds__(threads_for(AMODE), 1)
                 sm100::tmem_ld_wait(r);
                 if constexpr (FUSED) {
                     aux[1] = aux[0];
-                    epi_load_aux(p.epi, row, col0 + c + 32, row < p.M && c + 32 < BN && col0 + c + 64 <= p.N, aux[0]);
+                    if (c + 32 < BN) epi_load_aux(p.epi, row - lane, p.M, col0 + c + 32, p.N, aux[0]);
                     epi_chunk(p.epi, row - lane, p.M, col0 + c, p.N - col0 - c, r, aux[1], tile + EPI_TILE_BYTES / 4 + c,
                               tile);
                 } else if (row < p.M) {

@@ -78,7 +78,7 @@ struct PairConfig {
 
 template <typename OutT, int AMODE>
 __host__ __device__ constexpr int pair_epilogue_halves() {
-    return std::is_same<OutT, FusedOut>::value ? PairConfig<AMODE>::FUSED_HALVES : 1;
+    return FusedTraits<OutT>::fused ? PairConfig<AMODE>::FUSED_HALVES : 1;
 }
 template <typename OutT, int AMODE>
 __host__ __device__ constexpr int pair_threads() {
@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(pair_threads<OutT, AMODE>(), 1)
                           const ParamsFor<OutT> p) {
     using C = PairConfig<AMODE>;
     constexpr bool COMPACT = AMODE != A_TMA;
-    constexpr bool FUSED = std::is_same<OutT, FusedOut>::value;
+    constexpr bool FUSED = FusedTraits<OutT>::fused;
     static_assert(C::SUB == 1, "one 128-deep slab per stage");
     // Epilogue warps per lane quarter; half h takes the chunks whose place in the reading order is
     // h modulo HALVES, in filling a taken-over accumulator as in reading one.
@@ -566,13 +566,13 @@ __global__ void __launch_bounds__(pair_threads<OutT, AMODE>(), 1)
             const int row = tc.mb * C::BM + tile_row;
             const int col0 = tc.nb * C::BN;
             const bool regroup = XG && !hand_off && p.dst.n > 1;
-            [[maybe_unused]] AuxRaw aux[2];
+            [[maybe_unused]] AuxRaw<FusedTraits<OutT>::columns> aux[2];
             [[maybe_unused]] float* tile =
                 reinterpret_cast<float*>(epi_stg + (quarter + 4 * half) * (FUSED ? C::FUSED_EPI_WARP : 0));
             if constexpr (FUSED) {
                 if (!hand_off) {
                     const int fcol = col0 + 32 * (b ? half : C::BN / 32 - 1 - half);
-                    epi_load_aux(p.epi, row, fcol, row < p.M && fcol + 32 <= p.N, aux[0]);
+                    epi_load_aux(p.epi, row - lane, p.M, fcol, p.N, aux[0]);
                     epi_load_bias<C::BN / 32 / HALVES>(p.epi, fcol, (b ? 32 : -32) * HALVES, p.N, tile + EPI_TILE_BYTES / 4);
                 }
             }
@@ -638,7 +638,7 @@ __global__ void __launch_bounds__(pair_threads<OutT, AMODE>(), 1)
                 } else if constexpr (FUSED) {
                     aux[1] = aux[0];
                     const int ncol = col + (b ? 32 : -32) * HALVES;  // the warp's next chunk
-                    epi_load_aux(p.epi, row, ncol, row < p.M && j + HALVES < C::BN / 32 && ncol + 32 <= p.N, aux[0]);
+                    if (j + HALVES < C::BN / 32) epi_load_aux(p.epi, row - lane, p.M, ncol, p.N, aux[0]);
                     if (col < p.N)
                         epi_chunk(p.epi, row - lane, p.M, col, p.N - col, r, aux[1],
                                   tile + EPI_TILE_BYTES / 4 + j / HALVES * 32, tile);

@@ -76,6 +76,18 @@ def test_activations_and_aux(act, aux_op):
         check_rounded(got, *fused64(A, B, act, bias, aux, aux_op), ot, f"{act.name} {aux_op.name} {ot.name}")
 
 
+# Row and column layouts of the epilogue with an aux operand, whole and partial tiles, on the single-CTA tiles and the pair.
+@pytest.mark.parametrize("M,N,K", [(100, 264, 512), (257, 777, 256), (2500, 1544, 256), (3000, 3001, 128)])
+@pytest.mark.parametrize("ot,at", [(OutType.F32, OutType.F32), (OutType.F32, OutType.BF16), (OutType.BF16, OutType.BF16),
+                                   (OutType.F16, OutType.F32)])
+@pytest.mark.parametrize("pad", [0, 7])
+def test_aux_layouts(M, N, K, ot, at, pad):
+    A, B = Operand(M, K, 1.0, 41), Operand(N, K, K ** -0.5, 42)
+    bias, aux = _randn(N, seed=43), _randn(M, N + pad, seed=44, dtype=DTYPE[at])[:, :N]
+    got = _fused(A, B, ot, Act.SILU, bias, OutType.F32, aux, at, AuxOp.MUL)
+    check_rounded(got, *fused64(A, B, Act.SILU, bias, aux, AuxOp.MUL), ot, f"{M}x{N}")
+
+
 # Pitches and bases that allow wide accesses, 16-byte ones only by chance, or none.
 @pytest.mark.parametrize("ldd,offset", [(256, 0), (264, 8), (257, 0), (300, 1), (256, 3)])
 @pytest.mark.parametrize("ot", list(OutType))
