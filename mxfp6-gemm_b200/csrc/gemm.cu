@@ -37,9 +37,10 @@ thread_local int t_last_error = MXFP6_OK;
 thread_local long long t_wait_budget = 0;  // 0: the kernels' default (kern::WAIT_BUDGET)
 std::atomic<uint64_t> g_launches{0};
 
-// Tag of one stream-K launch, written into the workspace's hand-off flags: the flags are never
-// cleared, so a flag counts only when it holds this launch's tag. The high half is drawn once per
-// process, so stale flags from another process's use of the same memory do not match either.
+// Tag of one stream-K launch, written into the workspace's hand-off flags: a flag counts only when it
+// holds this launch's tag, so the workspace needs no initial contents. The CTA that took a hand-off over
+// clears its flag, for replays of the launch from a graph, which share its tag. The high half is drawn
+// once per process, so stale flags from another process's use of the same memory do not match either.
 uint64_t next_sk_epoch() {
     static std::atomic<uint64_t> counter{((uint64_t)std::random_device{}() << 32) | 1u};
     return counter.fetch_add(1, std::memory_order_relaxed);

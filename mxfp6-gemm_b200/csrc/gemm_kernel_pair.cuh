@@ -710,6 +710,9 @@ __global__ void __launch_bounds__(pair_threads<OutT, AMODE>(), 1)
         sm100::tc_fence_before();
         __syncthreads();
     }
+    // The hand-off this CTA took over is used up: clear its flag, so that a replay of this launch from a graph, whose tag is
+    // the same, does not take the flag for its own.
+    if (XF && work.take_over && threadIdx.x == 0) sm100::st_release_gpu_u64(p.sk_flags + 2 * (cluster_id - 1) + rank, 0);
     sm100::cluster_sync();  // no CTA leaves while its peer may still touch its shared memory
     if (warp == 1) {
         __syncwarp();

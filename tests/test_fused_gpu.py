@@ -119,6 +119,37 @@ def test_schedules(M, N, K, want):
     check_rounded(got, *ref, OutType.BF16, want + " without workspace")
 
 
+def test_stream_k_flags_are_used_up():
+    """A stream-K launch replayed from a graph has the tag of the capture: no flag of one replay may be left for the next,
+    which would take over accumulators that are not written yet."""
+    M, N, K = 4090, 3570, 6144
+    assert _route_of(OutType.BF16, M, N, K)["stream_k"]
+    A, B = Operand(M, K, 1.0, 9), Operand(N, K, K ** -0.5, 10)
+    n = lib.gemm_fused_workspace_size(M, N, A.Kp, A.row_bytes)
+    ws = torch.zeros(n, dtype=torch.uint8, device="cuda")
+    D = torch.empty(M, N, dtype=torch.bfloat16, device="cuda")
+    s = torch.cuda.Stream()
+
+    def call():
+        assert lib.gemm_fused(OutType.BF16, M, N, A.Kp, A.packed, B.packed, A.scales, B.scales, D, A.row_bytes, B.row_bytes,
+                              None, ws, n, stream=s) == lib.OK
+
+    s.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        call()
+    ref = fused64(A, B, Act.NONE, None, None, AuxOp.NONE)
+    pairs = lib.stream_k_bytes() // (256 * 256 * 4 + 16)
+    for _ in range(2):
+        D.fill_(0)
+        g.replay()
+        _finish()
+        check_rounded(D, *ref, OutType.BF16)
+        flags = ws[pairs * 256 * 256 * 4:pairs * (256 * 256 * 4 + 16)].view(torch.int64)
+        assert (flags == 0).all()
+        assert ws[:pairs * 256 * 256 * 4].any()  # accumulators were handed over
+
+
 @pytest.mark.parametrize("M,N,K,want", [(1, 128, 128, None), (33, 384, 160, None), (130, 512, 2048, None),
                                         (17, 2048, 4096, None), (64, 128, 256, None), (128, 640, 384, None), (200, 2048, 4096, "splits"), (2050, 6144, 512, None), (1500, 2048, 24576, "banded")])
 def test_quantised_output(M, N, K, want):
