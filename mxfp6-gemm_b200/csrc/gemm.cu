@@ -1008,9 +1008,9 @@ void run_validated(int ot, int M, int N, int Kp, const void* dA, const void* dB,
 // recorded, or M == 0).
 bool validate_fused(int M, int N, int Kp, const void* dA, const void* dB, const void* sA, const void* sB,
                     const void* dD, int Ar, int Br) {
-    if (M < 0 || N <= 0 || Kp <= 0 || Kp % K_TILE || N > (1 << 30)) {
+    if (M < 0 || N <= 0 || Kp <= 0 || Kp % K_TILE || M > (1 << 30) || N > (1 << 30)) {
         set_error(MXFP6_ERR_INVALID_SHAPE,
-                  "unsupported fused shape %dx%dx%d: M >= 0, N > 0 and Kp a positive multiple of %d (pad with kpad())",
+                  "unsupported fused shape %dx%dx%d: M in 0..2^30, N in 1..2^30 and Kp a positive multiple of %d (pad with kpad())",
                   M, N, Kp, K_TILE);
         return false;
     }

@@ -35,7 +35,7 @@ constexpr int MAX_TOKENS = 128, MAX_TOPK = 16, MAX_EXPERTS = 512;
 constexpr int MAX_SLOTS = MAX_TOKENS * MAX_TOPK;
 
 // Up to NMAX tokens of one expert: rows [start, start + n) of the sorted slots.
-struct Entry {
+struct __align__(16) Entry {
     int expert, start, n, pad;
 };
 
@@ -524,12 +524,17 @@ __global__ void __launch_bounds__(ProductConfig<KIND, NMAX>::THREADS, ProductCon
     constexpr bool EARLY = KIND == KIND_DOWN;
     if (!EARLY) sm100::griddep_wait();
     // the first item's entry is read beside the count (it exists in the workspace whatever the count is)
-    const Entry first = p.entries[blockIdx.x / p.tiles];
-    const int total = *p.n_entries * p.tiles;
+    // Past L1: its lines are only sure to be newer than the list after the wait.
+    auto entry = [&](int a) {
+        const int4 q = __ldcg(reinterpret_cast<const int4*>(p.entries) + a);
+        return Entry{q.x, q.y, q.z, q.w};
+    };
+    const Entry first = entry((int)blockIdx.x / p.tiles);
+    const int total = __ldcg(p.n_entries) * p.tiles;
     if (EARLY && warp != 0) sm100::griddep_wait();
     if (!EARLY || warp != 0) sm100::griddep_launch_dependents();
     // the entry of item `it`, read an item ahead of its use
-    auto entry_at = [&](int it) { return it < total ? p.entries[it / p.tiles] : Entry{0, 0, 0, 0}; };
+    auto entry_at = [&](int it) { return it < total ? entry(it / p.tiles) : Entry{0, 0, 0, 0}; };
     uint32_t issued_mask = 0, issued_phase = 0;
     bool mma_issued = false;
 
@@ -807,10 +812,10 @@ struct CombineParams {
 __global__ void __launch_bounds__(256) moe_combine(const CombineParams p) {
     sm100::griddep_launch_dependents();
     // the places and weights were complete when the down product let this kernel start (see moe_product): read them
-    // before the wait
+    // before the wait, past L1
     const int t = blockIdx.y, col = (blockIdx.x * blockDim.x + threadIdx.x) * 4, lane = threadIdx.x & 31;
-    const int slot = lane < p.top_k ? p.slot_of[t * p.top_k + lane] : -1;
-    const float weight = lane < p.top_k ? p.slot_w[t * p.top_k + lane] : 0.0f;
+    const int slot = lane < p.top_k ? __ldcg(p.slot_of + t * p.top_k + lane) : -1;
+    const float weight = lane < p.top_k ? __ldcg(p.slot_w + t * p.top_k + lane) : 0.0f;
     sm100::griddep_wait();
     float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     const bool in = col < p.hidden;

@@ -184,7 +184,8 @@ def test_quantised_output(M, N, K, want):
 
 
 # The compact strides of A (0.75*K with K % 128 != 0): re-padded into the workspace, or loaded in place.
-@pytest.mark.parametrize("M,N,K", [(5, 70, 96), (130, 300, 2080), (300, 2056, 480), (513, 520, 800)])
+@pytest.mark.parametrize("M,N,K", [(5, 70, 96), (130, 300, 2080), (300, 2056, 480), (513, 520, 800), (1500, 2056, 480),
+                                   (1500, 2003, 480), (1300, 1537, 288)])
 @pytest.mark.parametrize("ws", [True, False])
 def test_compact_a(M, N, K, ws):
     A, B = Operand(M, K, 1.0, 17, row_bytes=K * 3 // 4), Operand(N, K, K ** -0.5, 18)

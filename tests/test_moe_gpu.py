@@ -116,7 +116,9 @@ def _routed(layer, T, k, seed=0, ot=OutType.BF16, xt=None, renormalize=True, res
 @pytest.mark.parametrize("T,E,k,H,I", [(1, 1, 1, 128, 128), (1, 8, 2, 256, 384), (3, 64, 8, 512, 128), (7, 8, 2, 1024, 512),
                                        (16, 16, 4, 384, 256), (17, 4, 1, 256, 256), (40, 8, 2, 256, 640),
                                        (61, 60, 6, 512, 384), (128, 16, 8, 256, 256), (128, 2, 2, 384, 128),
-                                       (128, 64, 8, 128, 128), (2, 40, 16, 2048, 1408), (5, 512, 3, 128, 128)])
+                                       (128, 64, 8, 128, 128), (2, 40, 16, 2048, 1408), (5, 512, 3, 128, 128),
+                                       (20, 100, 5, 128, 128), (30, 200, 4, 128, 128), (128, 300, 16, 128, 128),
+                                       (17, 33, 16, 256, 128), (32, 7, 1, 640, 128), (4, 256, 8, 128, 256)])
 @pytest.mark.parametrize("gated", [True, False])
 def test_sizes(T, E, k, H, I, gated):
     _routed(Layer(E, H, I, gated), T, k, ot=OutType.F16)
@@ -128,6 +130,11 @@ def test_activations_and_types(act, renormalize):
     layer = Layer(6, 256, 256, act != Act.RELU, act)
     for ot, xt in ((OutType.F32, OutType.BF16), (OutType.BF16, OutType.F16), (OutType.F16, OutType.F32)):
         _routed(layer, 9, 2, ot=ot, xt=xt, renormalize=renormalize, residual=_randn(9, 256, seed=4, dtype=DTYPE[ot]))
+
+
+@pytest.mark.parametrize("T,E,k", [(1, 64, 8), (16, 64, 2), (40, 24, 6), (128, 130, 3)])
+def test_shares_of_the_whole_softmax(T, E, k):
+    _routed(Layer(E, 128, 128), T, k, seed=3, ot=OutType.F32, renormalize=False)
 
 
 def test_every_token_on_one_expert():
