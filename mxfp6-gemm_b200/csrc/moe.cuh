@@ -523,12 +523,12 @@ __global__ void __launch_bounds__(ProductConfig<KIND, NMAX>::THREADS, ProductCon
     // in warp 0, outputs in warps 2..5.
     constexpr bool EARLY = KIND == KIND_DOWN;
     if (!EARLY) sm100::griddep_wait();
-    // the first item's entry is read beside the count (it exists in the workspace whatever the count is)
-    // Past L1: its lines are only sure to be newer than the list after the wait.
+    // An entry, past L1: its lines are only sure to be newer than the list after the wait.
     auto entry = [&](int a) {
         const int4 q = __ldcg(reinterpret_cast<const int4*>(p.entries) + a);
         return Entry{q.x, q.y, q.z, q.w};
     };
+    // the first item's entry is read beside the count (it exists in the workspace whatever the count is)
     const Entry first = entry((int)blockIdx.x / p.tiles);
     const int total = __ldcg(p.n_entries) * p.tiles;
     if (EARLY && warp != 0) sm100::griddep_wait();
