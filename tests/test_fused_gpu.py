@@ -193,6 +193,21 @@ def test_compact_a(M, N, K, ws):
     check_rounded(got, *fused64(A, B, Act.GELU_TANH, None, None, AuxOp.NONE), OutType.F16)
 
 
+def test_compact_a_in_place_on_the_pair():
+    """The loader warps under the pair's fused epilogue: scratch off, no workspace, both epilogue layouts."""
+    prev = lib.set_repad_scratch(0)
+    try:
+        for N in (4704, 4699):
+            M, K = 4096, 224
+            assert _route_of(OutType.F16, M, N, K)["MT"] == 256
+            A, B = Operand(M, K, 1.0, 45, row_bytes=K * 3 // 4), Operand(N, K, K ** -0.5, 46)
+            bias, aux = _randn(N, seed=47), _randn(M, N, seed=48, dtype=torch.float16)
+            got = _fused(A, B, OutType.F16, Act.RELU, bias, OutType.F32, aux, OutType.F16, AuxOp.ADD, ws=False)
+            check_rounded(got, *fused64(A, B, Act.RELU, bias, aux, AuxOp.ADD), OutType.F16)
+    finally:
+        lib.set_repad_scratch(prev)
+
+
 def test_residual_in_place_and_null_epilogue():
     A, B = Operand(100, 256, 1.0, 19), Operand(192, 256, 0.06, 20)
     D = _randn(100, 192, seed=21, dtype=torch.bfloat16)

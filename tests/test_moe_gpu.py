@@ -264,6 +264,39 @@ def test_two_layers_in_a_graph():
         check()
 
 
+def test_two_streams_at_once():
+    """Two layers on two streams, each with its own workspace, beside few-row GEMMs on both: the results of the same
+    calls one after another."""
+    ot, T, k = OutType.F32, 24, 3
+    layers = [Layer(16, 256, 384, seed=80), Layer(16, 256, 256, False, Act.GELU, seed=90)]
+    A, B = Operand(20, 1024, 1.0, 91), Operand(640, 1024, 0.03, 92)
+    streams = [torch.cuda.Stream() for _ in layers]
+    xs = [_randn(T, 256, seed=100 + i) for i in range(2)]
+    gs = [_randn(T, 16, seed=110 + i) for i in range(2)]
+    spaces = [_space(layer, T, k) for layer in layers]
+    outs = [[torch.empty(T, 256, device="cuda") for _ in range(8)] for _ in layers]
+    ds = [[torch.empty(20, 640, device="cuda") for _ in range(8)] for _ in layers]
+
+    def call(i, r):
+        ws, n = spaces[i]
+        assert lib.moe(layers[i].layer, ot, T, k, xs[i], ot, outs[i][r], ws, n, logits=gs[i], stream=streams[i]) == lib.OK
+        assert lib.gemm_fused(ot, 20, 640, 1024, A.packed, B.packed, A.scales, B.scales, ds[i][r], 768, 768,
+                              stream=streams[i]) == lib.OK
+
+    torch.cuda.synchronize()
+    for i in range(2):
+        call(i, 0)
+        torch.cuda.synchronize()
+    for r in range(1, 8):
+        for i in range(2):
+            call(i, r)
+    torch.cuda.synchronize()
+    assert lib.device_status() == 0
+    for i in range(2):
+        for r in range(1, 8):
+            assert torch.equal(outs[i][r], outs[i][0]) and torch.equal(ds[i][r], ds[0][0])
+
+
 def test_prompt_and_decode_share_weights():
     """The layer's weights are GEMM operands as they are: one expert's up product through gemm_fused equals
     the layer's, for an expert without a gate and an identity-free comparison of the whole layer."""
