@@ -475,9 +475,9 @@ template <int BN, typename OutT, bool PARTIAL, int AMODE>
 bool launch_gemm(int M, int N, int Kp, const void* dA, const void* dB, const uint8_t* sA,
                  const uint8_t* sB, const kern::DstList& dl, float* ws, int A_row_bytes, int B_row_bytes,
                  int splits, cudaStream_t stream, const FusedLaunch* fused = nullptr) {
-    using C = kern::Config<BN, AMODE>;
+    using C = kern::Config<BN, AMODE, kern::FusedTraits<OutT>::fused, kern::FusedTraits<OutT>::columns>;
     auto kernel = kern::gemm_mxfp6_sm100<BN, OutT, PARTIAL, AMODE>;
-    constexpr int smem_bytes = kern::FusedTraits<OutT>::fused ? C::FUSED_SMEM_BYTES : C::SMEM_BYTES;
+    constexpr int smem_bytes = C::SMEM_BYTES;
     static std::once_flag attr_once[kMaxDevices];
     const int dev = current_device();
     if (dev < 0 || dev >= kMaxDevices) {
@@ -525,7 +525,7 @@ bool launch_gemm(int M, int N, int Kp, const void* dA, const void* dB, const uin
     const int grid = (int)(tiles < sm_count() ? tiles : sm_count());
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid, 1, 1);
-    cfg.blockDim = dim3(kern::threads_for(AMODE), 1, 1);
+    cfg.blockDim = dim3(C::THREADS, 1, 1);
     cfg.dynamicSmemBytes = smem_bytes;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];

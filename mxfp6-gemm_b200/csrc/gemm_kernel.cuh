@@ -56,10 +56,22 @@ constexpr int A_TMA_BYTES = BM * BK * 3 / 4;  // packed bytes one A slab moves
 // the one a launch uses. Drains after a timeout always use WAIT_BUDGET / 4.
 constexpr long long WAIT_BUDGET = 4000000000LL;
 
-template <int BN, int AMODE = A_TMA>
+// FUSED: a launch with a fused epilogue. With the tensor load's A it has two epilogue warps per lane quarter (HALVES),
+// which take the tile's chunks in turn: one warp per scheduler leaves the activation's latencies exposed, and there is no
+// second accumulator to hide them behind. 512 x 4096 x 1024 with residual 10.2 against 9.2 us, 1526 x 2304 x 1664 into
+// MXFP6 16.5 against 14.0 us, 140 x 2457 x 1248 in the column layout 11.3 against 9.7 us. In the row layout a quarter's
+// warps share one tile: only a width's last chunk goes through it, and that is always the same warp's. In the column
+// layout each warp has its own, for which 128 columns give up a ring stage, and 256 columns keep one warp per quarter (a
+// stage less there: 1000 x 4096 x 4096 22.5 -> 23.5 us).
+template <int BN, int AMODE = A_TMA, bool FUSED = false, bool COLUMNS = false>
 struct Config {
     static_assert(BN == 128 || BN == 256, "tile width");
-    static constexpr int STAGES = BN == 256 ? 4 : 6;
+    static constexpr int HALVES = FUSED && AMODE == A_TMA && !(COLUMNS && BN == 256) ? 2 : 1;
+    static constexpr int STAGES = (BN == 256 ? 4 : 6) - (COLUMNS && HALVES == 2 ? 1 : 0);
+    static constexpr int EPI_TILES = !FUSED ? 0 : COLUMNS ? 4 * HALVES : 4;
+    static constexpr int EPI_BIAS = FUSED ? BN / HALVES : 0;  // floats per epilogue warp
+    static constexpr int EPI_BYTES = EPI_TILES * EPI_TILE_BYTES + 4 * HALVES * EPI_BIAS * 4;
+    static constexpr int THREADS = threads_for(AMODE) + 128 * (HALVES - 1);
     static constexpr int A_BYTES = BM * BK;  // one byte per code in shared memory
     static constexpr int B_BYTES = BN * BK;
     static constexpr int AB_STAGE = A_BYTES + B_BYTES;
@@ -72,9 +84,8 @@ struct Config {
     static constexpr int TMEM_SFB = BN + 4;
     static constexpr int TMEM_COLS = BN == 256 ? 512 : 256;
     static constexpr int BAR_BYTES = 256;
-    static constexpr int SMEM_BYTES = 1024 + STAGES * (AB_STAGE + SF_STAGE) + BAR_BYTES;
-    static constexpr int FUSED_SMEM_BYTES = SMEM_BYTES + 4 * (EPI_TILE_BYTES + BN * 4);  // fused: tiles, biases
-    static_assert(FUSED_SMEM_BYTES <= 227 * 1024, "shared memory budget");
+    static constexpr int SMEM_BYTES = 1024 + STAGES * (AB_STAGE + SF_STAGE) + BAR_BYTES + EPI_BYTES;
+    static_assert(SMEM_BYTES <= 227 * 1024, "shared memory budget");
 };
 
 // Output destinations: D is written into each of n row-major [M][ldd] matrices at column col0
@@ -243,12 +254,12 @@ __device__ __forceinline__ void store_rows_regrouped(const DstList& dl, uint8_t*
 // AMODE (compact_a.cuh): A_TMA loads A with the 16U6 tensor load; A_CPASYNC adds four
 // loader warps that copy the A image from p.a_ptr (tmA unused).
 template <int BN, typename OutT, bool PARTIAL, int AMODE = A_TMA>
-__global__ void __launch_bounds__(threads_for(AMODE), 1)
+__global__ void __launch_bounds__(Config<BN, AMODE, FusedTraits<OutT>::fused, FusedTraits<OutT>::columns>::THREADS, 1)
     gemm_mxfp6_sm100(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                      const ParamsFor<OutT> p) {
-    using C = Config<BN, AMODE>;
     constexpr bool COMPACT = AMODE != A_TMA;
     constexpr bool FUSED = FusedTraits<OutT>::fused;
+    using C = Config<BN, AMODE, FUSED, FusedTraits<OutT>::columns>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     // 1024-byte alignment for the 128-byte-swizzled operand tiles.
     const uint32_t raw_u32 = sm100::smem_u32(smem_raw);
@@ -279,7 +290,7 @@ __global__ void __launch_bounds__(threads_for(AMODE), 1)
             sm100::mbar_init(empty_bar(s), 1);
         }
         sm100::mbar_init(acc_full, 1);
-        sm100::mbar_init(acc_empty, 4 * 32);
+        sm100::mbar_init(acc_empty, C::HALVES * 4 * 32);
         sm100::mbar_init(drain_bar, 1);
         *abort_flag = 0;
         sm100::fence_mbar_init();
@@ -431,6 +442,7 @@ __global__ void __launch_bounds__(threads_for(AMODE), 1)
     } else {
         // ---------------- epilogue (warps 2..5) ----------------
         const int quarter = warp & 3;  // tensor-memory lanes 32*quarter .. 32*quarter+31
+        const int half = C::HALVES > 1 ? (warp - EPI_WARP0) / 4 : 0;  // chunks half, half + HALVES, ... of the tile
         const uint32_t t_row = tmem_base + ((uint32_t)(32 * quarter) << 16);
         uint32_t acc_phase = 0;
         for (int t = blockIdx.x; t < total_tiles; t += gridDim.x) {
@@ -438,10 +450,14 @@ __global__ void __launch_bounds__(threads_for(AMODE), 1)
             const int row = tc.mb * BM + 32 * quarter + lane;
             const int col0 = tc.nb * BN;
             [[maybe_unused]] AuxRaw<FusedTraits<OutT>::columns> aux[2];
-            [[maybe_unused]] float* tile = reinterpret_cast<float*>(bar_ptr + C::BAR_BYTES + quarter * (EPI_TILE_BYTES + BN * 4));
+            [[maybe_unused]] float* tile =
+                reinterpret_cast<float*>(bar_ptr + C::BAR_BYTES) +
+                (C::EPI_TILES > 4 ? quarter + 4 * half : quarter) * (EPI_TILE_BYTES / 4);
+            [[maybe_unused]] float* biases = reinterpret_cast<float*>(bar_ptr + C::BAR_BYTES + C::EPI_TILES * EPI_TILE_BYTES) +
+                                             (quarter + 4 * half) * C::EPI_BIAS;
             if constexpr (FUSED) {
-                epi_load_aux(p.epi, row - lane, p.M, col0, p.N, aux[0]);
-                epi_load_bias<BN / 32>(p.epi, col0, 32, p.N, tile + EPI_TILE_BYTES / 4);
+                epi_load_aux(p.epi, row - lane, p.M, col0 + 32 * half, p.N, aux[0]);
+                epi_load_bias<BN / 32 / C::HALVES>(p.epi, col0 + 32 * half, 32 * C::HALVES, p.N, biases);
             }
             if (!sm100::wait_parity_bounded(acc_full, acc_phase, abort_flag, p.wait_budget)) {
                 if (!*abort_flag) raise_status(0x4u, abort_flag);
@@ -449,16 +465,17 @@ __global__ void __launch_bounds__(threads_for(AMODE), 1)
             }
             sm100::tc_fence_after();
 #pragma unroll 1
-            for (int c = 0; c < BN; c += 32) {
+            for (int c = 32 * half; c < BN; c += 32 * C::HALVES) {
                 if (col0 + c >= p.N) break;  // masked half tile (uniform across the warp)
                 uint32_t r[32];
                 sm100::tmem_ld_32x32b_x32(t_row + (uint32_t)c, r);
                 sm100::tmem_ld_wait(r);
                 if constexpr (FUSED) {
                     aux[1] = aux[0];
-                    if (c + 32 < BN) epi_load_aux(p.epi, row - lane, p.M, col0 + c + 32, p.N, aux[0]);
-                    epi_chunk(p.epi, row - lane, p.M, col0 + c, p.N - col0 - c, r, aux[1], tile + EPI_TILE_BYTES / 4 + c,
-                              tile);
+                    constexpr int step = 32 * C::HALVES;
+                    if (c + step < BN) epi_load_aux(p.epi, row - lane, p.M, col0 + c + step, p.N, aux[0]);
+                    epi_chunk(p.epi, row - lane, p.M, col0 + c, p.N - col0 - c, r, aux[1],
+                              biases + c / step * 32, tile);
                 } else if (row < p.M) {
                     if constexpr (PARTIAL) {
                         float* dst = p.ws + ((size_t)tc.split * p.M + row) * p.N + col0 + c;
