@@ -42,25 +42,33 @@ struct FewConfig {
     static_assert(stages(16) * stage_bytes(16) >= 16 * PITCH * 4 && 16 * 128 + stages(16) * W_BYTES >= 128 * 128, "ring");
 };
 
-// R rows of 32 columns: lane l has the sums of column n. `in`: the column is inside D.
+// The bias of a lane's column n and the aux values of R rows of it.
+struct FewOperands {
+    float bias, aux[FEW_BATCH];
+};
+// `in`: the column is inside D.
 template <int R>
-__device__ __forceinline__ void few_store(const Epi& e, int row0, int M, int n, bool in, float (&v)[R]) {
-    const int lane = threadIdx.x & 31;
-    if (e.bias && in) {
-        const float b = load_elem(e.bias, e.bias_type, (size_t)n);
-#pragma unroll
-        for (int i = 0; i < R; i++) v[i] += b;
-    }
-    float a[R];
+__device__ __forceinline__ void few_load(const Epi& e, int row0, int M, int n, bool in, FewOperands& o) {
+    o.bias = e.bias && in ? load_elem(e.bias, e.bias_type, (size_t)n) : 0.0f;
     if (e.aux_op != AUX_NONE) {
 #pragma unroll
         for (int i = 0; i < R; i++)
-            a[i] = in && row0 + i < M ? load_elem(e.aux, e.aux_type, (size_t)(row0 + i) * (size_t)e.ld_aux + (size_t)n) : 0.0f;
+            o.aux[i] = in && row0 + i < M ? load_elem(e.aux, e.aux_type, (size_t)(row0 + i) * (size_t)e.ld_aux + (size_t)n) : 0.0f;
+    }
+}
+
+// R rows of 32 columns: lane l has the sums of column n.
+template <int R>
+__device__ __forceinline__ void few_store(const Epi& e, int row0, int M, int n, bool in, float (&v)[R], const FewOperands& o) {
+    const int lane = threadIdx.x & 31;
+    if (e.bias) {
+#pragma unroll
+        for (int i = 0; i < R; i++) v[i] += o.bias;
     }
     activate_all<R>(e.act, v);
     if (e.aux_op != AUX_NONE) {
 #pragma unroll
-        for (int i = 0; i < R; i++) epi_join(e.aux_op, v[i], a[i]);
+        for (int i = 0; i < R; i++) epi_join(e.aux_op, v[i], o.aux[i]);
     }
     if (e.out_type != T_MXFP6) {
 #pragma unroll
@@ -69,28 +77,44 @@ __device__ __forceinline__ void few_store(const Epi& e, int row0, int M, int n, 
         return;
     }
     // MXFP6: a row's 32 columns are one block. Magnitudes order like their bits (NaN does not count); four lanes' codes
-    // make 24 bits, and six lanes write the block's 24 bytes.
+    // make 24 bits, and six lanes write the block's 24 bytes. Each step runs on all rows before the next one, rows past M
+    // included, so that their exchanges are in flight together.
+    uint32_t code[R], c24[R];
+#pragma unroll
+    for (int i = 0; i < R; i++) code[i] = __reduce_max_sync(0xffffffffu, v[i] != v[i] ? 0u : __float_as_uint(fabsf(v[i])));
 #pragma unroll
     for (int i = 0; i < R; i++) {
-        if (row0 + i >= M) break;
-        const uint32_t mag = v[i] != v[i] ? 0u : __float_as_uint(fabsf(v[i]));
-        const uint32_t code = scale_code(__uint_as_float(__reduce_max_sync(0xffffffffu, mag)));
-        const uint32_t c = to_e2m3x2(0.0f, v[i] * e8m0_reciprocal(code)) & 0x3Fu;
-        const uint32_t c12 = c | (__shfl_down_sync(0xffffffffu, c, 1) << 6);
-        const uint32_t c24 = c12 | (__shfl_down_sync(0xffffffffu, c12, 2) << 12);  // 24 bits in every fourth lane
-        const int first = lane * 4 / 3;                                            // group in which word `lane` starts
-        const uint32_t lo = __shfl_sync(0xffffffffu, c24, 4 * first), hi = __shfl_sync(0xffffffffu, c24, 4 * first + 4);
+        code[i] = scale_code(__uint_as_float(code[i]));
+        c24[i] = to_e2m3x2(0.0f, v[i] * e8m0_reciprocal(code[i])) & 0x3Fu;
+    }
+#pragma unroll
+    for (int i = 0; i < R; i++) c24[i] |= __shfl_down_sync(0xffffffffu, c24[i], 1) << 6;
+#pragma unroll
+    for (int i = 0; i < R; i++) c24[i] |= __shfl_down_sync(0xffffffffu, c24[i], 2) << 12;  // 24 bits in every fourth lane
+    const int first = lane * 4 / 3;  // group in which word `lane` starts
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+        const uint32_t lo = __shfl_sync(0xffffffffu, c24[i], 4 * first), hi = __shfl_sync(0xffffffffu, c24[i], 4 * first + 4);
         const uint32_t w = lane % 3 == 0 ? lo | (hi << 24) : lane % 3 == 1 ? (lo >> 8) | (hi << 16) : (lo >> 16) | (hi << 8);
+        if (row0 + i >= M) continue;
         uint8_t* d = static_cast<uint8_t*>(e.out) + (size_t)(row0 + i) * (size_t)e.ldd + (size_t)((n - lane) / 4 * 3);
         if (lane < 6) reinterpret_cast<uint32_t*>(d)[lane] = w;
-        if (lane == 6) e.scales[scale_atom_offset(row0 + i, (n - lane) / 32, e.k_atoms)] = (uint8_t)code;
+        if (lane == 6) e.scales[scale_atom_offset(row0 + i, (n - lane) / 32, e.k_atoms)] = (uint8_t)code[i];
     }
 }
 
-// This CTA's share of the tile: tasks of 32 columns of R rows, summed over the cluster's accumulators at `here` in segment
-// order. All of a task's loads are in flight together.
+// The first task of this warp (few_finish).
 template <int BN, int R>
-__device__ __forceinline__ void few_finish(const FusedParams& p, int tile, int rank, int S, uint32_t here) {
+__device__ __forceinline__ void few_load_first(const FusedParams& p, int tile, int rank, int S, FewOperands& o) {
+    constexpr int G = BN / 32;
+    const int t = rank + S * (int)(threadIdx.x >> 5), n = tile * BN + t % G * 32 + (int)(threadIdx.x & 31);
+    if (t < (p.M + R - 1) / R * G) few_load<R>(p.epi, t / G * R, p.M, n, n < p.N, o);
+}
+
+// This CTA's share of the tile: tasks of 32 columns of R rows, summed over the cluster's accumulators at `here` in segment
+// order. All of a task's loads are in flight together; `o` has the first task's bias and aux values.
+template <int BN, int R>
+__device__ __forceinline__ void few_finish(const FusedParams& p, int tile, int rank, int S, uint32_t here, FewOperands& o) {
     using C = FewConfig<BN>;
     constexpr int G = BN / 32;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -100,6 +124,7 @@ __device__ __forceinline__ void few_finish(const FusedParams& p, int tile, int r
     const int tasks = (p.M + R - 1) / R * G;
     for (int t = rank + S * warp; t < tasks; t += S * (FEW_THREADS / 32)) {
         const int row0 = t / G * R, c = t % G * 32 + lane, n = tile * BN + c;
+        if (t >= S * (FEW_THREADS / 32)) few_load<R>(p.epi, row0, p.M, n, n < p.N, o);
         if (n - lane >= p.N) continue;
         const uint32_t at = (uint32_t)(row0 * C::PITCH + c) * 4u;
         float q[FEW_CLUSTER][R], v[R];
@@ -115,7 +140,7 @@ __device__ __forceinline__ void few_finish(const FusedParams& p, int tile, int r
             for (int s = 1; s < FEW_CLUSTER; s++)
                 if (s < S) v[i] += q[s][i];
         }
-        few_store<R>(p.epi, row0, p.M, n, n < p.N, v);
+        few_store<R>(p.epi, row0, p.M, n, n < p.N, v, o);
     }
 }
 
@@ -227,6 +252,12 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
         if (ok) sm100::tc_commit(acc_full);
     }
     __syncwarp();
+    // The first task's bias and aux values are on their way while the last MMAs run.
+    FewOperands first = {};
+    if (p.M <= FEW_SINGLE)
+        few_load_first<BN, 1>(p, tile, rank, S, first);
+    else
+        few_load_first<BN, FEW_BATCH>(p, tile, rank, S, first);
     // The accumulator to shared memory: a lane per row, half of the columns per warp.
     const bool got = sm100::wait_parity_bounded(acc_full, 0, abort_flag, p.wait_budget);
     if (!got && !*abort_flag) raise_status(0x4u, abort_flag);
@@ -266,9 +297,9 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
     }
     if (S > 1) sm100::cluster_sync();
     if (p.M <= FEW_SINGLE)
-        few_finish<BN, 1>(p, tile, rank, S, sm100::smem_u32(acc));
+        few_finish<BN, 1>(p, tile, rank, S, sm100::smem_u32(acc), first);
     else
-        few_finish<BN, FEW_BATCH>(p, tile, rank, S, sm100::smem_u32(acc));
+        few_finish<BN, FEW_BATCH>(p, tile, rank, S, sm100::smem_u32(acc), first);
     if (S > 1) sm100::cluster_sync();  // no CTA leaves while another may read its accumulator
 }
 
