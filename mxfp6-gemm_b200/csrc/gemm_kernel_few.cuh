@@ -20,7 +20,8 @@ namespace kern {
 constexpr int FEW_ROWS = 64;       // rows at most
 constexpr int FEW_CLUSTER = 8;     // K segments at most
 constexpr int FEW_THREADS = 256;
-// Rows a warp finishes together: one up to FEW_SINGLE rows, where there are more warps than groups of four, else four.
+// Rows of a column that a warp finishes together: one up to FEW_SINGLE rows, where there are more warps than groups of
+// four, else four.
 constexpr int FEW_BATCH = 4, FEW_SINGLE = 16;
 
 template <int BN>
@@ -42,14 +43,14 @@ struct FewConfig {
     static_assert(stages(16) * stage_bytes(16) >= 16 * PITCH * 4 && 16 * 128 + stages(16) * W_BYTES >= 128 * 128, "ring");
 };
 
-// The bias of a lane's column n and the aux values of R rows of it.
+// Bias and aux values of a task: of R rows of a lane's column, or of four columns of a row (few_quad).
 struct FewOperands {
-    float bias, aux[FEW_BATCH];
+    float bias[4], aux[FEW_BATCH];
 };
 // `in`: the column is inside D.
 template <int R>
 __device__ __forceinline__ void few_load(const Epi& e, int row0, int M, int n, bool in, FewOperands& o) {
-    o.bias = e.bias && in ? load_elem(e.bias, e.bias_type, (size_t)n) : 0.0f;
+    o.bias[0] = e.bias && in ? load_elem(e.bias, e.bias_type, (size_t)n) : 0.0f;
     if (e.aux_op != AUX_NONE) {
 #pragma unroll
         for (int i = 0; i < R; i++)
@@ -60,47 +61,18 @@ __device__ __forceinline__ void few_load(const Epi& e, int row0, int M, int n, b
 // R rows of 32 columns: lane l has the sums of column n.
 template <int R>
 __device__ __forceinline__ void few_store(const Epi& e, int row0, int M, int n, bool in, float (&v)[R], const FewOperands& o) {
-    const int lane = threadIdx.x & 31;
     if (e.bias) {
 #pragma unroll
-        for (int i = 0; i < R; i++) v[i] += o.bias;
+        for (int i = 0; i < R; i++) v[i] += o.bias[0];
     }
     activate_all<R>(e.act, v);
     if (e.aux_op != AUX_NONE) {
 #pragma unroll
         for (int i = 0; i < R; i++) epi_join(e.aux_op, v[i], o.aux[i]);
     }
-    if (e.out_type != T_MXFP6) {
 #pragma unroll
-        for (int i = 0; i < R; i++)
-            if (in && row0 + i < M) store_elem(e.out, e.out_type, (size_t)(row0 + i) * (size_t)e.ldd + (size_t)n, v[i]);
-        return;
-    }
-    // MXFP6: a row's 32 columns are one block. Magnitudes order like their bits (NaN does not count); four lanes' codes
-    // make 24 bits, and six lanes write the block's 24 bytes. Each step runs on all rows before the next one, rows past M
-    // included, so that their exchanges are in flight together.
-    uint32_t code[R], c24[R];
-#pragma unroll
-    for (int i = 0; i < R; i++) code[i] = __reduce_max_sync(0xffffffffu, v[i] != v[i] ? 0u : __float_as_uint(fabsf(v[i])));
-#pragma unroll
-    for (int i = 0; i < R; i++) {
-        code[i] = scale_code(__uint_as_float(code[i]));
-        c24[i] = to_e2m3x2(0.0f, v[i] * e8m0_reciprocal(code[i])) & 0x3Fu;
-    }
-#pragma unroll
-    for (int i = 0; i < R; i++) c24[i] |= __shfl_down_sync(0xffffffffu, c24[i], 1) << 6;
-#pragma unroll
-    for (int i = 0; i < R; i++) c24[i] |= __shfl_down_sync(0xffffffffu, c24[i], 2) << 12;  // 24 bits in every fourth lane
-    const int first = lane * 4 / 3;  // group in which word `lane` starts
-#pragma unroll
-    for (int i = 0; i < R; i++) {
-        const uint32_t lo = __shfl_sync(0xffffffffu, c24[i], 4 * first), hi = __shfl_sync(0xffffffffu, c24[i], 4 * first + 4);
-        const uint32_t w = lane % 3 == 0 ? lo | (hi << 24) : lane % 3 == 1 ? (lo >> 8) | (hi << 16) : (lo >> 16) | (hi << 8);
-        if (row0 + i >= M) continue;
-        uint8_t* d = static_cast<uint8_t*>(e.out) + (size_t)(row0 + i) * (size_t)e.ldd + (size_t)((n - lane) / 4 * 3);
-        if (lane < 6) reinterpret_cast<uint32_t*>(d)[lane] = w;
-        if (lane == 6) e.scales[scale_atom_offset(row0 + i, (n - lane) / 32, e.k_atoms)] = (uint8_t)code[i];
-    }
+    for (int i = 0; i < R; i++)
+        if (in && row0 + i < M) store_elem(e.out, e.out_type, (size_t)(row0 + i) * (size_t)e.ldd + (size_t)n, v[i]);
 }
 
 // The first task of this warp (few_finish).
@@ -141,6 +113,95 @@ __device__ __forceinline__ void few_finish(const FusedParams& p, int tile, int r
                 if (s < S) v[i] += q[s][i];
         }
         few_store<R>(p.epi, row0, p.M, n, n < p.N, v, o);
+    }
+}
+
+// The same for aligned rows and MXFP6, in tasks of four rows of 32 columns with four columns of a row per lane: a fourth of
+// the exchange's loads, wide stores, and a block's maximum and codes in eight lanes (64 x 8192 x 2048 into MXFP6 11.6
+// against 9.2 us, 36 x 3328 x 1408 with residual 8.7 / 7.3, 16 x 8192 x 2048 7.2 / 6.8; one row 6.98 / 7.08, so it keeps
+// the other form).
+__device__ __forceinline__ void few_quad_load(const Epi& e, int row, int M, int n, int valid, FewOperands& o) {
+    if (e.bias) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) o.bias[i] = i < valid ? load_elem(e.bias, e.bias_type, (size_t)(n + i)) : 0.0f;
+    }
+    if (e.aux_op == AUX_NONE) return;
+    const size_t at = (size_t)row * (size_t)e.ld_aux + (size_t)n;
+    if (!e.aux_vec || valid < 4 || row >= M) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) o.aux[i] = i < valid && row < M ? load_elem(e.aux, e.aux_type, at + i) : 0.0f;
+    } else if (e.aux_type == T_F32) {
+        const float4 q = *reinterpret_cast<const float4*>(static_cast<const float*>(e.aux) + at);
+        o.aux[0] = q.x;
+        o.aux[1] = q.y;
+        o.aux[2] = q.z;
+        o.aux[3] = q.w;
+    } else {
+        const uint2 q = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(e.aux) + at);
+        unpack2(q.x, e.aux_type, o.aux[0], o.aux[1]);
+        unpack2(q.y, e.aux_type, o.aux[2], o.aux[3]);
+    }
+}
+
+template <int BN>
+__device__ __forceinline__ void few_quad(const FusedParams& p, int tile, int rank, int S, uint32_t here, FewOperands& o) {
+    using C = FewConfig<BN>;
+    constexpr int G = BN / 32;
+    const Epi& e = p.epi;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint32_t part[FEW_CLUSTER];
+#pragma unroll
+    for (int s = 0; s < FEW_CLUSTER; s++) part[s] = s < S ? sm100::mapa_shared(here, (uint32_t)s) : 0u;
+    const int tasks = (p.M + 3) / 4 * G;
+    for (int t = rank + S * warp; t < tasks; t += S * (FEW_THREADS / 32)) {
+        const int row = t / G * 4 + lane / 8, c = t % G * 32 + lane % 8 * 4, n = tile * BN + c;
+        if (t >= S * (FEW_THREADS / 32)) few_quad_load(e, row, p.M, n, p.N - n, o);
+        if (tile * BN + t % G * 32 >= p.N) continue;
+        const uint32_t at = (uint32_t)(row * C::PITCH + c) * 4u;
+        float4 q[FEW_CLUSTER];
+#pragma unroll
+        for (int s = 0; s < FEW_CLUSTER; s++)
+            q[s] = s < S && row < p.M ? sm100::ld_cluster_f32x4(part[s] + at) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float v[4] = {q[0].x, q[0].y, q[0].z, q[0].w};
+#pragma unroll
+        for (int s = 1; s < FEW_CLUSTER; s++)
+            if (s < S) {
+                v[0] += q[s].x;
+                v[1] += q[s].y;
+                v[2] += q[s].z;
+                v[3] += q[s].w;
+            }
+        if (e.bias) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] += o.bias[i];
+        }
+        activate_all<4>(e.act, v);
+        if (e.aux_op != AUX_NONE) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) epi_join(e.aux_op, v[i], o.aux[i]);
+        }
+        if (e.out_type != T_MXFP6) {
+            if (row < p.M && n < p.N) store_elems4(e, row, n, p.N - n, v);
+            continue;
+        }
+        // magnitudes order like their bits (NaN does not count)
+        uint32_t mag = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) mag = max(mag, v[i] != v[i] ? 0u : __float_as_uint(fabsf(v[i])));
+#pragma unroll
+        for (int x = 1; x < 8; x *= 2) mag = max(mag, __shfl_xor_sync(0xffffffffu, mag, x));
+        const uint32_t code = scale_code(__uint_as_float(mag));
+        const float inv = e8m0_reciprocal(code);
+        const uint32_t c4 = __byte_perm(to_e2m3x2(v[1] * inv, v[0] * inv), to_e2m3x2(v[3] * inv, v[2] * inv), 0x5410) & 0x3F3F3F3Fu;
+        const uint32_t c24 = __dp4a(c4, 0x00004001u, 0u) + (__dp4a(c4, 0x40010000u, 0u) << 12);
+        // lane j of the block's eight: bytes [3j, 3j + 3); words 0..5 from lanes 4j/3 and the next one
+        const int j = lane % 8, first = (lane & 24) + j * 4 / 3;
+        const uint32_t lo = __shfl_sync(0xffffffffu, c24, first), hi = __shfl_sync(0xffffffffu, c24, first + 1);
+        const uint32_t w = j % 3 == 0 ? lo | (hi << 24) : j % 3 == 1 ? (lo >> 8) | (hi << 16) : (lo >> 16) | (hi << 8);
+        if (row >= p.M) continue;
+        uint8_t* d = static_cast<uint8_t*>(e.out) + (size_t)row * (size_t)e.ldd + (size_t)((n - 4 * j) / 4 * 3);
+        if (j < 6) reinterpret_cast<uint32_t*>(d)[j] = w;
+        if (j == 6) e.scales[scale_atom_offset(row, (n - 4 * j) / 32, e.k_atoms)] = (uint8_t)code;
     }
 }
 
@@ -254,7 +315,11 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
     __syncwarp();
     // The first task's bias and aux values are on their way while the last MMAs run.
     FewOperands first = {};
-    if (p.M <= FEW_SINGLE)
+    const bool quad = p.epi.out_type == T_MXFP6 || (p.epi.out_vec && p.M > 1);
+    if (quad) {
+        const int t = rank + S * warp, row = t / (BN / 32) * 4 + lane / 8, n = tile * BN + t % (BN / 32) * 32 + lane % 8 * 4;
+        if (t < (p.M + 3) / 4 * (BN / 32)) few_quad_load(p.epi, row, p.M, n, p.N - n, first);
+    } else if (p.M <= FEW_SINGLE)
         few_load_first<BN, 1>(p, tile, rank, S, first);
     else
         few_load_first<BN, FEW_BATCH>(p, tile, rank, S, first);
@@ -296,7 +361,9 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
         sm100::tmem_dealloc(tmem_base, C::TMEM_COLS);
     }
     if (S > 1) sm100::cluster_sync();
-    if (p.M <= FEW_SINGLE)
+    if (quad)
+        few_quad<BN>(p, tile, rank, S, sm100::smem_u32(acc), first);
+    else if (p.M <= FEW_SINGLE)
         few_finish<BN, 1>(p, tile, rank, S, sm100::smem_u32(acc), first);
     else
         few_finish<BN, FEW_BATCH>(p, tile, rank, S, sm100::smem_u32(acc), first);
