@@ -7,6 +7,32 @@
 
 namespace mxfp6 {
 
+// Two floats in one 64-bit register: multiply, add and multiply-add take one instruction for both.
+struct F2 {
+    unsigned long long w;
+};
+__device__ __forceinline__ F2 pair(float a, float b) {
+    F2 r;
+    asm("mov.b64 %0, {%1,%2};" : "=l"(r.w) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ F2 both(float a) { return pair(a, a); }
+__device__ __forceinline__ void split(F2 x, float& a, float& b) { asm("mov.b64 {%0,%1}, %2;" : "=f"(a), "=f"(b) : "l"(x.w)); }
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
+    F2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.w) : "l"(a.w), "l"(b.w));
+    return r;
+}
+__device__ __forceinline__ F2 operator+(F2 a, F2 b) {
+    F2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.w) : "l"(a.w), "l"(b.w));
+    return r;
+}
+__device__ __forceinline__ F2 fma(F2 a, F2 b, F2 c) {
+    F2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.w) : "l"(a.w), "l"(b.w), "l"(c.w));
+    return r;
+}
 // E8M0 code of the smallest power of two >= v (v > 0, finite or +Inf): from the float bits,
 // the same result as frexp-based rounding up (a power of two maps to itself).
 __device__ __forceinline__ uint32_t ceil_pow2_code(float v) {
@@ -86,8 +112,9 @@ __device__ __forceinline__ void quantize16(const float* v, float inv, bool nan, 
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             uint16_t d;
-            asm("cvt.rn.satfinite.e2m3x2.f32 %0, %1, %2;" : "=h"(d) : "f"(fmaf(v[2 * i + 1], inv, 0.0f)),
-                "f"(fmaf(v[2 * i], inv, 0.0f)));
+            float lo, hi;
+            split(fma(pair(v[2 * i], v[2 * i + 1]), both(inv), both(0.0f)), lo, hi);
+            asm("cvt.rn.satfinite.e2m3x2.f32 %0, %1, %2;" : "=h"(d) : "f"(hi), "f"(lo));
             q[i] = d;
         }
     }
