@@ -107,15 +107,19 @@ __device__ __forceinline__ F2 activate(float v0, float v1) {
     return over_one_plus_ex2(v, v * both(-LOG2E));
 }
 
-template <int N>
+// Values of one row in pairs; a pair's shared reciprocal makes the last bit of one depend on the other. EACH: values of
+// different rows, each by itself, so that no row's result depends on another row.
+template <int N, bool EACH = false>
 __device__ __forceinline__ void activate_all(int act, float (&v)[N]) {
+    static_assert(EACH || N % 2 == 0, "pairs");
     switch (act) {
-#define MXFP6_ACT_CASE(A)                                                            \
-    case A:                                                                          \
-        _Pragma("unroll") for (int i = 0; i < N; i += 2) {                           \
-            float odd;                                                               \
-            split(activate<A>(v[i], v[i + 1 < N ? i + 1 : i]), v[i], i + 1 < N ? v[i + 1 < N ? i + 1 : i] : odd); \
-        }                                                                            \
+#define MXFP6_ACT_CASE(A)                                                              \
+    case A:                                                                            \
+        _Pragma("unroll") for (int i = 0; i < N; i += EACH ? 1 : 2) {                  \
+            float other;                                                               \
+            const F2 h = activate<A>(v[i], v[EACH ? i : i + 1]);                       \
+            split(h, v[i], EACH ? other : v[EACH ? i : i + 1]);                        \
+        }                                                                              \
         break;
         MXFP6_ACT_CASE(ACT_RELU)
         MXFP6_ACT_CASE(ACT_GELU)
@@ -318,7 +322,8 @@ __device__ __forceinline__ void epi_join(int op, float& v, float a) {
 constexpr int EPI_TILE_PITCH = 36;
 constexpr int EPI_TILE_BYTES = 32 * EPI_TILE_PITCH * 4;
 
-// The warp's rows of the last, partial chunk from its shared-memory tile, lane = column, eight rows at a time.
+// The warp's rows of the last, partial chunk from its shared-memory tile, lane = column, four rows at a time (the
+// code of eight, inlined into the chunk loop, costs whole chunks 1.5 us of 2048 x 6144 x 2048 with residual).
 // `in`: the lane's column is inside D.
 template <int OT>
 __device__ __forceinline__ void epi_rows(const Epi& e, int row0, int rows, int col, bool in, float bias,
@@ -327,37 +332,37 @@ __device__ __forceinline__ void epi_rows(const Epi& e, int row0, int rows, int c
     Out* out = static_cast<Out*>(e.out) + (size_t)row0 * (size_t)e.ldd + (size_t)col;
     size_t ai = (size_t)row0 * (size_t)e.ld_aux + (size_t)col;
 #pragma unroll 1
-    for (int q = 0; q < rows; q += 8) {
-        float v[8], a[8];
+    for (int q = 0; q < rows; q += 4) {
+        float v[4], a[4];
 #pragma unroll
-        for (int k = 0; k < 8; k++) a[k] = 0.0f;
+        for (int k = 0; k < 4; k++) a[k] = 0.0f;
         if (e.aux_op != AUX_NONE) {
             if (e.aux_type == T_F32) {
 #pragma unroll
-                for (int k = 0; k < 8; k++)
+                for (int k = 0; k < 4; k++)
                     if (in && q + k < rows) a[k] = load_elem(e.aux, T_F32, ai + (size_t)k * (size_t)e.ld_aux);
             } else if (e.aux_type == T_F16) {
 #pragma unroll
-                for (int k = 0; k < 8; k++)
+                for (int k = 0; k < 4; k++)
                     if (in && q + k < rows) a[k] = load_elem(e.aux, T_F16, ai + (size_t)k * (size_t)e.ld_aux);
             } else {
 #pragma unroll
-                for (int k = 0; k < 8; k++)
+                for (int k = 0; k < 4; k++)
                     if (in && q + k < rows) a[k] = load_elem(e.aux, T_BF16, ai + (size_t)k * (size_t)e.ld_aux);
             }
         }
 #pragma unroll
-        for (int k = 0; k < 8; k++) v[k] = tile[(q + k) * EPI_TILE_PITCH] + bias;
-        activate_all<8>(e.act, v);
+        for (int k = 0; k < 4; k++) v[k] = tile[(q + k) * EPI_TILE_PITCH] + bias;
+        activate_all<4, true>(e.act, v);
         if (e.aux_op != AUX_NONE) {
 #pragma unroll
-            for (int k = 0; k < 8; k++) v[k] = e.aux_op == AUX_ADD ? v[k] + a[k] : v[k] * a[k];
+            for (int k = 0; k < 4; k++) v[k] = e.aux_op == AUX_ADD ? v[k] + a[k] : v[k] * a[k];
         }
 #pragma unroll
-        for (int k = 0; k < 8; k++)
+        for (int k = 0; k < 4; k++)
             if (in && q + k < rows) store_elem(out + (size_t)k * (size_t)e.ldd, OT, 0, v[k]);
-        out += (size_t)8 * (size_t)e.ldd;
-        ai += (size_t)8 * (size_t)e.ld_aux;
+        out += (size_t)4 * (size_t)e.ldd;
+        ai += (size_t)4 * (size_t)e.ld_aux;
     }
 }
 

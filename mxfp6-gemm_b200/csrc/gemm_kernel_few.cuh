@@ -65,7 +65,7 @@ __device__ __forceinline__ void few_store(const Epi& e, int row0, int M, int n, 
 #pragma unroll
         for (int i = 0; i < R; i++) v[i] += o.bias[0];
     }
-    activate_all<R>(e.act, v);
+    activate_all<R, true>(e.act, v);
     if (e.aux_op != AUX_NONE) {
 #pragma unroll
         for (int i = 0; i < R; i++) epi_join(e.aux_op, v[i], o.aux[i]);

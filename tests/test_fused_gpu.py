@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import mxfp6_b200 as lib
-from fused_ref import DTYPE, Operand, check_quantised, check_rounded, fused64
+from fused_ref import DTYPE, Operand, act64, check_quantised, check_rounded, fused64
 from mxfp6_b200 import Act, AuxOp, OutType
 
 pytestmark = pytest.mark.gpu
@@ -242,6 +242,46 @@ def test_special_values():
         fine = ref.isfinite() & (ref.abs() < 1e30)
         fine[:, 4] = False
         assert (got[fine].double() - ref[fine]).abs().max() < 1e-4
+
+
+@pytest.mark.parametrize("M", [1, 5, 20, 130, 1030])
+@pytest.mark.parametrize("N", [256, 257])
+def test_values_beside_each_other(M, N):
+    """Every ordered pair of extreme values in neighbouring columns: two values share a reciprocal."""
+    inf, nan = float("inf"), float("nan")
+    some = torch.tensor([0.0, -0.0, 1e-30, 0.7, -0.7, 6.5, -6.5, -8.0, 20.0, -44.0, 60.0, -90.0, 3e38, -3e38, inf, -inf])
+    pairs = torch.stack([some[:, None].expand(16, 16), some[None].expand(16, 16)], -1)
+    A, B = Operand(M, 128, 0.0, 40), Operand(N, 128, 1.0, 41)
+    for first, poison in ((0, False), (1, False), (0, True)):
+        v = torch.cat([pairs[:, 0:8], pairs[:, 8:16]])[16 * first:16 * first + 16].reshape(-1)
+        v = torch.cat([v, torch.zeros(N - 256)])
+        if poison:
+            v[::2] = nan
+        v = v.cuda()
+        for act in Act:
+            got = _fused(A, B, OutType.F32, act, v)
+            assert (got == got[0]).logical_or(got.isnan()).all()
+            got, x = got[0].double(), v.double()
+            assert (got.isnan() == x.isnan()).all()
+            low = x == -inf if act != Act.NONE else torch.zeros_like(x, dtype=torch.bool)
+            fine = x.isfinite() & (x.abs() < 1e9)
+            assert (got[low].abs() < 1e-16).all() and (got[x == inf] == inf).all()
+            assert (got[x == 3e38] > 2.9e38).all() and (act == Act.NONE or (got[x == -3e38].abs() < 1e-16).all())
+            # 2^-20 of the value as in fused64, and the 1e-17 that the negative tails end at
+            assert ((got - act64(act, x)).abs() <= 2.0 ** -20 * x.abs() + 1e-17)[fine].all(), act
+
+
+@pytest.mark.parametrize("M,N", [(6, 33), (20, 33), (40, 128), (200, 260), (300, 513)])
+def test_rows_do_not_depend_on_each_other(M, N):
+    A, B = Operand(M, 256, 2.0, 42), Operand(N, 256, 0.2, 43)
+    order = torch.from_numpy(np.random.default_rng(44).permutation(M))
+    P = Operand(M, 256, 2.0, 42)
+    P.packed = A.packed[order.cuda()].contiguous()
+    x = np.random.default_rng(42).standard_normal((M, 256), dtype=np.float32) * np.float32(2.0)
+    q = lib.quantize_to_mxfp6(x[order.numpy()])
+    P.scales = torch.from_numpy(lib.preprocess_scale(lib.pad_scales_k(q.scales, M, 256), M, 256)).cuda()
+    for act in Act:
+        assert torch.equal(_fused(P, B, OutType.F32, act), _fused(A, B, OutType.F32, act)[order.cuda()]), act
 
 
 def test_empty_and_stream():
