@@ -29,7 +29,7 @@ struct Epi {
     uint8_t* scales;    // MXFP6: tiled scales
     long long ld_aux, ldd;
     int bias_type, act, aux_op, aux_type, out_type;
-    int aux_vec;            // 16-byte loads of whole aux chunks are aligned
+    int aux_vec;            // 16-byte (1) or 32-byte (2) loads of whole aux chunks are aligned
     int out_vec;            // so are 16-byte (1) or 32-byte (2) stores; 0: neither, or aux is not
     int k_atoms;                     // MXFP6: N / 128
 };
@@ -298,6 +298,13 @@ __device__ __forceinline__ void epi_load_aux(const Epi& e, int row0, int M, int 
         }
     }
 }
+// 32 bytes in one load: with a lane per row, a load costs the cache one look-up per lane whatever its width.
+__device__ __forceinline__ void ld_v8(const uint4* s, uint4& a, uint4& b) {
+    asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w)
+                 : "l"(s)
+                 : "memory");
+}
 __device__ __forceinline__ void epi_load_aux(const Epi& e, int row0, int M, int col, int N, AuxRaw<false>& a) {
     const int row = row0 + (threadIdx.x & 31);
     const bool live = row < M && col >= 0 && col + 32 <= N;
@@ -305,6 +312,15 @@ __device__ __forceinline__ void epi_load_aux(const Epi& e, int row0, int M, int 
     const size_t i = (size_t)row * (size_t)e.ld_aux + (size_t)col;
     const uint4* s = e.aux_type == T_F32 ? reinterpret_cast<const uint4*>(static_cast<const float*>(e.aux) + i)
                                          : reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(e.aux) + i);
+    if (e.aux_vec == 2) {
+        ld_v8(s, a.q[0], a.q[1]);
+        ld_v8(s + 2, a.q[2], a.q[3]);
+        if (e.aux_type == T_F32) {
+            ld_v8(s + 4, a.q[4], a.q[5]);
+            ld_v8(s + 6, a.q[6], a.q[7]);
+        }
+        return;
+    }
 #pragma unroll
     for (int k = 0; k < 4; k++) a.q[k] = s[k];
     if (e.aux_type == T_F32) {

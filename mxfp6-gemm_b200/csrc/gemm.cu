@@ -421,7 +421,8 @@ bool validate_epilogue(const mxfp6_epilogue* ep, int M, int N, kern::Epi& e) {
         e.ld_aux = ep->ld_aux;
         e.aux_type = ep->aux_type;
         e.aux_op = ep->aux_op;
-        e.aux_vec = aligned(ep->aux, 16) && (M <= 1 || ep->ld_aux * type_bytes(ep->aux_type) % 16 == 0);
+        const long long pitch = M <= 1 ? 0 : ep->ld_aux * type_bytes(ep->aux_type);
+        e.aux_vec = aligned(ep->aux, 32) && pitch % 32 == 0 ? 2 : aligned(ep->aux, 16) && pitch % 16 == 0 ? 1 : 0;
     }
     e.bias = ep->bias;
     e.bias_type = ep->bias_type;
