@@ -526,10 +526,14 @@ __device__ __forceinline__ void epi_chunk(const Epi& e, int row0, int M, int col
     uint32_t w[6];
     quantize16(v, inv, nan0, w[0], w[1], w[2]);
     quantize16(v + 16, inv, nan1, w[3], w[4], w[5]);
-    uint2* d = reinterpret_cast<uint2*>(static_cast<uint8_t*>(e.out) + (size_t)row * (size_t)e.ldd + (size_t)(col / 4 * 3));
-    d[0] = make_uint2(w[0], w[1]);
-    d[1] = make_uint2(w[2], w[3]);
-    d[2] = make_uint2(w[4], w[5]);
+    uint8_t* d = static_cast<uint8_t*>(e.out) + (size_t)row * (size_t)e.ldd + (size_t)(col / 4 * 3);
+    if (col & 32) {  // 24 bytes from an odd multiple of 8 on, else from a multiple of 16
+        *reinterpret_cast<uint2*>(d) = make_uint2(w[0], w[1]);
+        *reinterpret_cast<uint4*>(d + 8) = make_uint4(w[2], w[3], w[4], w[5]);
+    } else {
+        *reinterpret_cast<uint4*>(d) = make_uint4(w[0], w[1], w[2], w[3]);
+        *reinterpret_cast<uint2*>(d + 16) = make_uint2(w[4], w[5]);
+    }
     e.scales[scale_atom_offset(row, col / 32, e.k_atoms)] = (uint8_t)code;
 }
 
