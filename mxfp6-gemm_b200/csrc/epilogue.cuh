@@ -62,27 +62,32 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // NaN stays NaN
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
-// 1/a and 1/b with one reciprocal, from 1/(ab): a and b in [1, 2^63], and their order within the pair turned round.
+// 1/a and 1/b. SHARE: with one reciprocal, from 1/(ab), for a and b in [1, 2^63].
+template <bool SHARE>
 __device__ __forceinline__ F2 rcp(float a, float b) {
+    if constexpr (!SHARE) return pair(rcp(a), rcp(b));
     return both(rcp(a * b)) * pair(b, a);
 }
 
 // v / (1 + 2^y) for two values, y <= 62 or NaN where v is.
+template <bool SHARE>
 __device__ __forceinline__ F2 over_one_plus_ex2(F2 v, F2 y) {
     float a, b;
     split(ex2(y) + both(1.0f), a, b);
-    return v * rcp(fminf(a, 0x1p63f), fminf(b, 0x1p63f));  // a NaN must not reach the other value
+    if constexpr (!SHARE) return v * rcp<false>(a, b);
+    return v * rcp<true>(fminf(a, 0x1p63f), fminf(b, 0x1p63f));  // a NaN must not reach the other value
 }
 
 // v Phi(v) = max(v, 0) - |v| erfc(|v| / sqrt(2)) / 2, with erfc(x) = (a1 t + ... + a5 t^5) e^(-x^2), t = 1 / (1 + p x)
 // (Hastings; Abramowitz and Stegun 7.1.26: absolute error 1.5e-7; the coefficients here are halved, and
 // e^(-x^2) = 2^(-v^2 log2(e) / 2)). From |v| = 16 on the second term is 0 in FP32.
+template <bool SHARE>
 __device__ __forceinline__ F2 gelu_erf(float v0, float v1) {
     const float u0 = fminf(fabsf(v0), 16.0f), u1 = fminf(fabsf(v1), 16.0f);
     const F2 u = pair(u0, u1);
     float a, b;
     split(fma(u, both(0.3275911f * 0.70710678118654752f), both(1.0f)), a, b);
-    const F2 t = rcp(a, b);
+    const F2 t = rcp<SHARE>(a, b);
     F2 q = fma(t, both(0.5f * 1.061405429f), both(0.5f * -1.453152027f));
     q = fma(q, t, both(0.5f * 1.421413741f));
     q = fma(q, t, both(0.5f * -0.284496736f));
@@ -93,33 +98,34 @@ __device__ __forceinline__ F2 gelu_erf(float v0, float v1) {
 
 // The quotients have no cancellation anywhere, so they stay within a few FP32 ulp. Below -43 (-7.5) SiLU (the tanh form of
 // GELU) is the value there, -9e-18 (-4e-18), instead of one even nearer to 0: 1 + e^43 is what the shared reciprocal takes.
-template <int ACT>
+template <int ACT, bool SHARE>
 __device__ __forceinline__ F2 activate(float v0, float v1) {
     if constexpr (ACT == ACT_RELU) return pair(max_nan(v0, 0.0f), max_nan(v1, 0.0f));
-    if constexpr (ACT == ACT_GELU) return gelu_erf(v0, v1);
+    if constexpr (ACT == ACT_GELU) return gelu_erf<SHARE>(v0, v1);
     if constexpr (ACT == ACT_GELU_TANH) {
         // 0.5 v (1 + tanh(u)) = v / (1 + e^(-2u)), u = sqrt(2/pi) (v + 0.044715 v^3)
         const F2 v = pair(max_nan(v0, -7.5f), max_nan(v1, -7.5f));
         constexpr float c = -LOG2E * 1.5957691216057308f;
-        return over_one_plus_ex2(v, v * fma(v * v, both(c * 0.044715f), both(c)));
+        return over_one_plus_ex2<SHARE>(v, v * fma(v * v, both(c * 0.044715f), both(c)));
     }
     const F2 v = pair(max_nan(v0, -43.0f), max_nan(v1, -43.0f));
-    return over_one_plus_ex2(v, v * both(-LOG2E));
+    return over_one_plus_ex2<SHARE>(v, v * both(-LOG2E));
 }
 
 // Values of one row in pairs; a pair's shared reciprocal makes the last bit of one depend on the other. EACH: values of
-// different rows, each by itself, so that no row's result depends on another row.
+// different rows, each with its own, so that no row's result depends on another row.
 template <int N, bool EACH = false>
 __device__ __forceinline__ void activate_all(int act, float (&v)[N]) {
-    static_assert(EACH || N % 2 == 0, "pairs");
+    static_assert(N % 2 == 0 || (N == 1 && EACH), "pairs");
     switch (act) {
-#define MXFP6_ACT_CASE(A)                                                              \
-    case A:                                                                            \
-        _Pragma("unroll") for (int i = 0; i < N; i += EACH ? 1 : 2) {                  \
-            float other;                                                               \
-            const F2 h = activate<A>(v[i], v[EACH ? i : i + 1]);                       \
-            split(h, v[i], EACH ? other : v[EACH ? i : i + 1]);                        \
-        }                                                                              \
+#define MXFP6_ACT_CASE(A)                                                  \
+    case A:                                                                \
+        _Pragma("unroll") for (int i = 0; i < N; i += 2) {                 \
+            float a, b;                                                    \
+            split(activate<A, !EACH>(v[i], v[N > 1 ? i + 1 : i]), a, b);   \
+            v[i] = a;                                                      \
+            if (N > 1) v[N > 1 ? i + 1 : i] = b;                           \
+        }                                                                  \
         break;
         MXFP6_ACT_CASE(ACT_RELU)
         MXFP6_ACT_CASE(ACT_GELU)
