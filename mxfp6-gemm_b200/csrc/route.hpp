@@ -230,16 +230,21 @@ inline Route route_for(int M, int N, int Kp, int sms, int min_splits = 1) {
 // apply. One wave: the tiles of 128 columns times the segments fit two CTAs per SM, with room for the clusters that do
 // not fill a group of SMs (40 clusters of 7 on 148 SMs took two waves: 13.6 us against 8.6 us as clusters of 4). Wider
 // matrices take tiles of 256 columns, one per SM. Measured against the GEMM kernels with their split-K reduce (BF16, bias
-// and SiLU, back to back): 1 x 4096 x 4096 6.8 against 8.7 us, 16 x 8192 x 2048 7.5 / 11.4, 32 x 4096 x 4096 8.1 / 8.9,
-// 64 x 8192 x 2048 9.6 / 11.0; 64 x 4096 x 4096 9.7 / 8.7, 64 x 2048 x 8192 10.4 / 8.9, 128 x 4096 x 4096 13.1 / 10.9: what
-// grows with the rows is the exchange of the segments' sums.
+// and SiLU, back to back): 1 x 4096 x 4096 6.2 against 8.7 us, 16 x 8192 x 2048 6.9 / 10.4, 32 x 4096 x 4096 8.1 / 9.1,
+// 64 x 8192 x 2048 8.7 / 10.4, 64 x 2048 x 2048 7.9 / 9.9, 128 x 4096 x 4096 13.1 / 10.8.
+//
+// What grows with the rows is the exchange of the segments' sums, and the segments are 8 at most. So with 8 of them the
+// GEMM kernels take over above 40 rows where they split K (from 20 slabs on) and the tiles' clusters fill the SMs:
+// 48 x 2048 x 4096 8.0 against 7.2 us, 64 x 2560 x 2560 8.9 / 7.0, 64 x 4096 x 4096 9.9 / 8.6 (48 x 4096 x 8192 10.9 / 11.4;
+// 11 tiles: 48 x 1408 x 6144 7.7 / 7.8, 64 x 1024 x 4096 7.2 / 7.4), and above 16 rows where K is very deep:
+// 24 x 1024 x 16384 10.3 / 9.1 (24 x 2560 x 10240 9.5 / 10.1).
 inline Route few_route(int M, int N, int Kp, int sms, int min_splits) {
     Route r{128, 128, 0};
     if (M < 1 || M > 64 || N < 1 || Kp < 128) return r;
     const int slabs = Kp / 128, narrow = (N - 1) / 128 + 1, wide = (N - 1) / 256 + 1;
     for (int s = 8; s >= 1; s /= 2)
         if (s >= min_splits && slabs >= 2 * s - 1 && narrow <= (2 * sms - 4 * s) / s) {
-            r.splits = s;
+            if (s < 8 || !((M > 40 && slabs >= 20 && narrow >= 12) || (M > 16 && slabs >= 96))) r.splits = s;
             return r;
         }
     r.NT = 256;

@@ -284,6 +284,19 @@ def test_rows_do_not_depend_on_each_other(M, N):
         assert torch.equal(_fused(P, B, OutType.F32, act), _fused(A, B, OutType.F32, act)[order.cuda()]), act
 
 
+# Around the rows where the few-row kernel hands over, with a last chunk that ends inside a lane's four columns or not.
+@pytest.mark.parametrize("M", [1, 2, 15, 17, 40, 41, 64, 65])
+@pytest.mark.parametrize("N,K", [(1608, 2560), (1606, 640), (100, 12416)])
+@pytest.mark.parametrize("ot", list(OutType))
+def test_few_rows(M, N, K, ot):
+    A, B = Operand(M, K, 1.0, 50), Operand(N, K, K ** -0.5, 51)
+    bias, aux = _randn(N, seed=52), _randn(M, N, seed=53, dtype=DTYPE[ot])
+    for act, op in ((Act.GELU, AuxOp.ADD), (Act.SILU, AuxOp.MUL), (Act.NONE, AuxOp.NONE)):
+        a = None if op == AuxOp.NONE else aux
+        got = _fused(A, B, ot, act, bias, aux=a, aux_type=ot, aux_op=op)
+        check_rounded(got, *fused64(A, B, act, bias, a, op), ot, f"{M}x{N}x{K}")
+
+
 def test_empty_and_stream():
     A, B = Operand(40, 256, 1.0, 26), Operand(64, 256, 0.06, 27)
     n0 = lib.launch_count()
