@@ -832,8 +832,8 @@ bool run(int ot, const Route& r, int M, int N, int Kp, const void* dA, const voi
 }
 
 // Route for an output type: FP32 output keeps split segments short enough for its tolerance.
-Route route_for_out(int ot, int M, int N, int Kp) {
-    return route_for(M, N, Kp, sm_count(), ot == MXFP6_OUT_F32 ? fp32_min_splits(Kp) : 1);
+Route route_for_out(int ot, int M, int N, int Kp, bool fused = false) {
+    return route_for(M, N, Kp, sm_count(), ot == MXFP6_OUT_F32 ? fp32_min_splits(Kp) : 1, fused);
 }
 
 // Bytes of a padded copy of A (rows of 0.75*Kp) placed after the split-K partials in the
@@ -949,7 +949,7 @@ void run_validated(int ot, int M, int N, int Kp, const void* dA, const void* dB,
             return;
         }
     }
-    Route r = route_for_out(ot, M, N, Kp);
+    Route r = route_for_out(ot, M, N, Kp, fused != nullptr);
     const int sms = sm_count();
     const int Nw = fused ? partials_pitch(N) : N;  // columns of the split-K partials
     if (r.splits > 1 || r.stream_k) {
@@ -1417,7 +1417,7 @@ size_t mxfp6_gemm_fused_workspace_size(int M, int N, int Kp, int A_row_bytes) {
     if (M <= 0 || N <= 0 || Kp <= 0 || Kp % K_TILE) return 0;
     size_t need = 0;
     for (int ot : {MXFP6_OUT_F16, MXFP6_OUT_F32}) {
-        const size_t b = route_ws_bytes(route_for_out(ot, M, N, Kp), M, partials_pitch(N), sm_count());
+        const size_t b = route_ws_bytes(route_for_out(ot, M, N, Kp, true), M, partials_pitch(N), sm_count());
         if (b > need) need = b;
     }
     const bool tma_stride = A_row_bytes % 32 == 0 && (long long)A_row_bytes >= (long long)Kp * 3 / 4;

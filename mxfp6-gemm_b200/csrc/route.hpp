@@ -30,7 +30,8 @@
 // (measured: the pair sustains a little more over several waves, the narrow tile streams A at
 // half the work per byte).
 // The cheapest candidate wins (a later candidate must win by 3%). gemm_workspace_size() and
-// gemm() both call route_for(), so the workspace a caller sizes always matches what is used.
+// gemm() both call route_for(), so the workspace a caller sizes always matches what is used. The fused
+// calls and their workspace query pass `fused`, which prices the reduce pass lower.
 #include <cstddef>
 
 namespace mxfp6 {
@@ -110,14 +111,18 @@ inline bool pair_stream_k_pays(long long tiles, int splits, long long slots, int
            (slots - tiles % slots) * (long long)k_slabs >= (long long)STREAM_K_MIN_SLABS * slots;
 }
 
-inline double route_cost_us(int M, int N, int Kp, int MT, int NT, int S, int sms) {
+inline double route_cost_us(int M, int N, int Kp, int MT, int NT, int S, int sms, bool fused = false) {
     const double HBM = 6.5e6;  // bytes per us
     // Fixed cost of a launch beyond the 128x128 kernel's, and of the split-K reduce's own launch,
     // in the model's units. Measured back to back on small shapes, where they dominate: 128x128
     // takes 6-8 us per call, 128x256 about 0.5 us more, the CTA pair about 4 us more, and a split
     // about 5 us more. On those shapes the slab terms read about 1.7x short, so the fixed terms
     // are scaled down by the same factor to keep the two comparable.
-    const double T_REDUCE_LAUNCH = 3.0;
+    // A fused call's epilogue is exposed after an unsplit tile and rides on the reduce's loads after a split one, so a
+    // split there costs less: with 1 for the reduce, 100 x 2560 x 2048 takes 7.9 us in 4 segments against 10.3 in one,
+    // 384 x 2048 x 4096 12.1 in 3 against 16.1, 700 x 512 x 2560 8.9 in 3 against 12.0 (BF16, bias and GELU), and the next
+    // better number of segments of the same tile wins by 1% (128 x 2048 x 8192: 10.1 us in 8, 10.9 in 6).
+    const double T_REDUCE_LAUNCH = fused ? 1.0 : 3.0;
     double t_slab, t_tile, t_fixed;
     int per_unit;
     if (MT == 256) {
@@ -184,14 +189,14 @@ inline int fp32_min_splits(int Kp) {
     return s < 1 ? 1 : (s > 32 ? 32 : s);
 }
 
-inline Route route_for(int M, int N, int Kp, int sms, int min_splits = 1) {
+inline Route route_for(int M, int N, int Kp, int sms, int min_splits = 1, bool fused = false) {
     Route best{128, N >= 256 ? 256 : 128, 1};
     if (M <= 0 || N <= 0 || Kp < 128 || sms <= 0) return best;
     const int slabs = Kp / 128;
     if (min_splits > slabs) min_splits = slabs;
     if (min_splits < 1) min_splits = 1;
     best.splits = min_splits;
-    double best_t = route_cost_us(M, N, Kp, best.MT, best.NT, min_splits, sms);
+    double best_t = route_cost_us(M, N, Kp, best.MT, best.NT, min_splits, sms, fused);
     const int shapes[3][2] = {{256, 256}, {128, 256}, {128, 128}};
     bool first = true;
     for (const auto& sh : shapes) {
@@ -200,8 +205,8 @@ inline Route route_for(int M, int N, int Kp, int sms, int min_splits = 1) {
         int s_max = slabs / 4 < 32 ? slabs / 4 : 32;  // every segment keeps >= 4 slabs
         if (s_max < min_splits) s_max = min_splits;
         for (int S = min_splits; S <= (s_max > 1 ? s_max : 1); S++) {
-            const double t = route_cost_us(M, N, Kp, MT, NT, S, sms);
-            if (first || t < best_t * 0.97) {
+            const double t = route_cost_us(M, N, Kp, MT, NT, S, sms, fused);
+            if (first || t < best_t * (fused && best.MT == MT && best.NT == NT ? 0.99 : 0.97)) {
                 best_t = t;
                 best = Route{MT, NT, S};
                 first = false;
@@ -230,13 +235,13 @@ inline Route route_for(int M, int N, int Kp, int sms, int min_splits = 1) {
 // apply. One wave: the tiles of 128 columns times the segments fit two CTAs per SM, with room for the clusters that do
 // not fill a group of SMs (40 clusters of 7 on 148 SMs took two waves: 13.6 us against 8.6 us as clusters of 4). Wider
 // matrices take tiles of 256 columns, one per SM. Measured against the GEMM kernels with their split-K reduce (BF16, bias
-// and SiLU, back to back): 1 x 4096 x 4096 6.2 against 8.7 us, 16 x 8192 x 2048 6.9 / 10.4, 32 x 4096 x 4096 8.1 / 9.1,
-// 64 x 8192 x 2048 8.7 / 10.4, 64 x 2048 x 2048 7.9 / 9.9, 128 x 4096 x 4096 13.1 / 10.8.
+// and SiLU, back to back): 1 x 4096 x 4096 6.2 against 8.7 us, 16 x 8192 x 2048 6.9 / 9.1, 32 x 4096 x 4096 8.1 / 9.1,
+// 64 x 8192 x 2048 8.7 / 10.3, 128 x 4096 x 4096 13.1 / 10.8.
 //
 // What grows with the rows is the exchange of the segments' sums, and the segments are 8 at most. So with 8 of them the
-// GEMM kernels take over above 40 rows where they split K (from 20 slabs on) and the tiles' clusters fill the SMs:
-// 48 x 2048 x 4096 8.0 against 7.2 us, 64 x 2560 x 2560 8.9 / 7.0, 64 x 4096 x 4096 9.9 / 8.6 (48 x 4096 x 8192 10.9 / 11.4;
-// 11 tiles: 48 x 1408 x 6144 7.7 / 7.8, 64 x 1024 x 4096 7.2 / 7.4), and above 16 rows where K is very deep:
+// GEMM kernels take over above 40 rows where the tiles' clusters fill the SMs: 48 x 2048 x 2048 7.2 against 6.8 us,
+// 64 x 2560 x 2560 8.9 / 7.0, 64 x 4096 x 4096 9.9 / 8.7 (40 x 2048 x 2048 6.8 / 6.8, 48 x 4096 x 8192 10.8 / 11.3;
+// 11 tiles: 48 x 1408 x 6144 7.7 / 7.7, 8 tiles: 64 x 1024 x 4096 7.2 / 7.4), and above 16 rows where K is very deep:
 // 24 x 1024 x 16384 10.3 / 9.1 (24 x 2560 x 10240 9.5 / 10.1).
 inline Route few_route(int M, int N, int Kp, int sms, int min_splits) {
     Route r{128, 128, 0};
@@ -244,7 +249,7 @@ inline Route few_route(int M, int N, int Kp, int sms, int min_splits) {
     const int slabs = Kp / 128, narrow = (N - 1) / 128 + 1, wide = (N - 1) / 256 + 1;
     for (int s = 8; s >= 1; s /= 2)
         if (s >= min_splits && slabs >= 2 * s - 1 && narrow <= (2 * sms - 4 * s) / s) {
-            if (s < 8 || !((M > 40 && slabs >= 20 && narrow >= 12) || (M > 16 && slabs >= 96))) r.splits = s;
+            if (s < 8 || !((M > 40 && narrow >= 12) || (M > 16 && slabs >= 96))) r.splits = s;
             return r;
         }
     r.NT = 256;
