@@ -440,7 +440,7 @@ __global__ void __launch_bounds__(Config<BN, AMODE, FusedTraits<OutT>::fused, Fu
         }
         sm100::cp_async_wait_all();
     } else {
-        // ---------------- epilogue (warps 2..5) ----------------
+        // ---------------- epilogue (warps 2..5, with two per quarter 2..9) ----------------
         const int quarter = warp & 3;  // tensor-memory lanes 32*quarter .. 32*quarter+31
         const int half = C::HALVES > 1 ? (warp - EPI_WARP0) / 4 : 0;  // chunks half, half + HALVES, ... of the tile
         const uint32_t t_row = tmem_base + ((uint32_t)(32 * quarter) << 16);

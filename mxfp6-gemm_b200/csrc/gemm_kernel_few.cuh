@@ -8,8 +8,8 @@
 //     memory of the cluster instead of global memory and a second kernel: each CTA leaves its FP32 accumulator in its own
 //     shared memory (over the operand ring, which is idle by then) and, after a cluster barrier, sums a share of the
 //     tile's (row, 32 columns) groups over the S CTAs, in segment order;
-//   * the epilogue runs on those groups with a lane per column, spread over all warps of all CTAs. In the tensor-memory
-//     layout (a lane per row) 16 rows would leave every warp but one idle.
+//   * the epilogue runs on those groups with a lane per column, or per four columns of a row, spread over all warps of
+//     all CTAs. In the tensor-memory layout (a lane per row) 16 rows would leave every warp but one idle.
 // Rows past M come from whatever follows A's rows in shared memory (any bytes are valid codes) and end in accumulator
 // lanes nobody reads. Waits are bounded (gemm_kernel.cuh); after a timeout every thread still takes both cluster barriers.
 #include "gemm_kernel.cuh"
