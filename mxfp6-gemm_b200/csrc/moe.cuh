@@ -624,6 +624,8 @@ __global__ void __launch_bounds__(ProductConfig<KIND, NMAX>::THREADS, ProductCon
                         ok = false;
                         break;
                     }
+                    // the scale warp's cp.async writes are generic-proxy writes; tcgen05.cp reads through the async proxy
+                    if constexpr (C::GATED) sm100::fence_async_shared();
                     const uint32_t sf = sf_base + stage * C::SF_BYTES;
                     sm100::tc_cp_32x128b_warpx4(tmem_base + C::TMEM_SFA, sm100::make_sf_desc(sf));
                     sm100::tc_cp_32x128b_warpx4(tmem_base + C::TMEM_SFB, sm100::make_sf_desc(sf + 512));

@@ -319,3 +319,33 @@ def test_prompt_and_decode_share_weights():
     ref, tol = layer.reference(x, ids, torch.ones(T, 1, device="cuda"))
     check_rounded(y, ref, tol, OutType.F32)
     check_rounded(out, ref, tol, OutType.F32)
+
+
+@pytest.mark.parametrize("T,k,E", [(1, 8, 64), (40, 2, 8), (61, 6, 64)])
+def test_weight_scales_of_every_slab(T, k, E):
+    """Weight scales that differ by up to 2^40 from one 128-column slab to the next, over many more slabs than stages: a
+    product with a scale of the stage's previous slab would be far off. Every call gives the same bits."""
+    H, I = 4096, 128
+    layer = Layer(E, H, I, act=Act.NONE, seed=120)
+    rng = np.random.default_rng(121)
+    R1 = E * 2 * I
+    # one slab of every eight counts, at a place of its own for each row; the others are 2^-40 of it
+    live = rng.integers(0, 8, (R1, 1)) == np.arange(H // 128)[None] % 8
+    raw = np.where(np.repeat(live, 4, 1), 124, 84).astype(np.uint8)
+    layer.W1.scales = torch.from_numpy(lib.preprocess_scale(raw, R1, H)).cuda()
+    layer.W1.values = values(layer.W1.packed.cpu().numpy(), raw, R1, H)
+    layer.w1 = layer.W1.values.view(E, 2 * I, H)
+    layer.layer = lib.MoELayer(E, H, I, layer.W1.packed, layer.W1.scales, layer.W2.packed, layer.W2.scales, True, Act.NONE)
+    x = _randn(T, H, seed=122)
+    ids = torch.stack([torch.randperm(E, generator=torch.Generator().manual_seed(t))[:k] for t in range(T)]).int().cuda()
+    w = _randn(T, k, seed=123)
+    first = _moe(layer, OutType.F32, x, OutType.F32, k, ids=ids, weights=w)
+    check_rounded(first, *layer.reference(x, ids, w), OutType.F32)
+    ws, n = _space(layer, T, k)
+    outs = [torch.empty_like(first) for _ in range(20)]
+    for _ in range(10):
+        for out in outs:
+            assert lib.moe(layer.layer, OutType.F32, T, k, x, OutType.F32, out, ws, n, ids=ids, weights=w) == lib.OK
+        torch.cuda.synchronize()
+        assert all(torch.equal(out, first) for out in outs)
+    assert lib.device_status() == 0
