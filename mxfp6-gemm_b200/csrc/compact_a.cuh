@@ -20,12 +20,14 @@
 // lane l writing word l % 4 of slot (l / 4) XOR (r % 8) (all 32 banks; word 3 is the zero gap,
 // a zero-fill copy) from the row's 96 contiguous packed bytes. Each thread signals a slab with
 // cp.async.mbarrier.arrive.noinc right after issuing it and moves on to the next stage; the
-// stage's full barrier completes when every copy has landed. Rows at or past M are skipped
-// (their outputs are not stored).
+// stage's full barrier completes when every copy has landed. These are generic-proxy writes, and the
+// MMAs read through the async proxy: the thread that waits on the full barrier fences the proxies
+// (the MMA thread, and in the pair's second CTA the relay). Rows at or past M are skipped (their
+// outputs are not stored).
 //
-// Measured on B200 (8192 x 8192 x 8160, FP16 out): 1.51 PFLOP/s, 0.57 of the same GEMM on a
-// padded A through the tensor load (2.65 PFLOP/s). Alternatives that were built and measured
-// slower: loader threads waiting for their own copies before a proxy fence and a barrier arrive
+// Measured on B200 (8192 x 8192 x 8160, FP16 out): 1.40 PFLOP/s, 0.50 of the same GEMM on a
+// padded A through the tensor load (2.83 PFLOP/s); 1.51 without the proxy fences, which the memory
+// model asks for. Alternatives that were built and measured slower: loader threads waiting for their own copies before a proxy fence and a barrier arrive
 // (0.30); raw rows staged in shared memory by tensor loads from a row-pair tensor map and expanded
 // there (0.33-0.39: two extra shared-memory passes, and every slab then waits on a store, a
 // proxy fence and eight warp arrivals before the MMAs may read it); 8-byte global loads into a

@@ -380,6 +380,8 @@ __global__ void __launch_bounds__(Config<BN, AMODE, FusedTraits<OutT>::fused, Fu
                         break;
                     }
                     sm100::tc_fence_after();
+                    // the loaders' cp.async writes are generic-proxy writes; the MMAs read through the async proxy
+                    if constexpr (COMPACT) sm100::fence_async_shared();
                     const uint32_t sf_src = sf_base + stage * C::SF_STAGE;
                     sm100::tc_cp_32x128b_warpx4(tmem_base + C::TMEM_SFA, sm100::make_sf_desc(sf_src));
 #pragma unroll

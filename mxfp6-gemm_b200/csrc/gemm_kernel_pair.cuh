@@ -402,6 +402,8 @@ __global__ void __launch_bounds__(pair_threads<OutT, AMODE>(), 1)
                         ok = false;
                         break;
                     }
+                    // the loaders' cp.async writes are generic-proxy writes; the MMAs read through the async proxy
+                    if constexpr (COMPACT) sm100::fence_async_shared();
                     const uint32_t sf_src = sf_base + stage * C::SF_STAGE;
                     // A's atom: one broadcast copy; B's two atoms, staged four times over: one wide copy
                     sm100::tc_cp_32x128b_warpx4_pair(tmem_base + C::TMEM_SFA, sm100::make_sf_desc(sf_src));
@@ -442,6 +444,7 @@ __global__ void __launch_bounds__(pair_threads<OutT, AMODE>(), 1)
                         ok = false;
                         break;
                     }
+                    sm100::fence_async_shared();  // this CTA's half of A, as in the leader
                     sm100::mbar_arrive_cluster(sm100::mapa_shared(full_bar(stage), 0));
                     if (++stage == C::STAGES) {
                         stage = 0;

@@ -384,3 +384,26 @@ def test_feed_forward_block(T, H, I):
     x.copy_(_randn(T, H, seed=35, dtype=torch.bfloat16))
     g.replay()
     check()
+
+
+@pytest.mark.parametrize("M,N,K", [(130, 300, 2080), (1500, 2056, 2080), (4096, 4704, 2016)])
+def test_compact_a_in_place_repeats(M, N, K):
+    """The loader warps refill each stage many times: every call gives the bits of the tensor load's A."""
+    prev = lib.set_repad_scratch(0)
+    try:
+        A, B = Operand(M, K, 1.0, 60, row_bytes=K * 3 // 4), Operand(N, K, K ** -0.5, 61)
+        P = Operand(M, K, 1.0, 60)
+        want = _fused(P, B, OutType.F32, Act.RELU, ws=False)
+        first = _fused(A, B, OutType.F32, Act.RELU, ws=False)
+        check_rounded(first, *fused64(A, B, Act.RELU, None, None, AuxOp.NONE), OutType.F32)
+        assert torch.equal(first, want)
+        ep = lib.Epilogue(act=Act.RELU)
+        outs = [torch.empty(M, N, device="cuda") for _ in range(8)]
+        for _ in range(10):
+            for D in outs:
+                assert lib.gemm_fused(OutType.F32, M, N, A.Kp, A.packed, B.packed, A.scales, B.scales, D, A.row_bytes,
+                                      B.row_bytes, ep) == lib.OK
+            _finish()
+            assert all(torch.equal(D, first) for D in outs)
+    finally:
+        lib.set_repad_scratch(prev)
