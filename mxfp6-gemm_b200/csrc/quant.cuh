@@ -71,8 +71,8 @@ __device__ __forceinline__ uint32_t scale_code(float m) {
 // x86-64) and -0.0 -> +0.0 (code 0; other negatives that round to zero keep the sign, 0x20).
 // Returns code(b) | code(a) << 8.
 __device__ __forceinline__ uint32_t to_e2m3x2(float a, float b) {
-    a = a != a ? 4.0f : a + 0.0f;
-    b = b != b ? 4.0f : b + 0.0f;
+    a = a != a ? 4.0f : __fadd_rn(a, 0.0f);  // never joined with the multiplication before it (quantize16)
+    b = b != b ? 4.0f : __fadd_rn(b, 0.0f);
     uint16_t d;
     asm("cvt.rn.satfinite.e2m3x2.f32 %0, %1, %2;" : "=h"(d) : "f"(a), "f"(b));
     return d;
@@ -99,9 +99,11 @@ __device__ __forceinline__ float max_abs16(const float* v, bool& nan) {
     return m;
 }
 
-// 16 values times `inv`, as 16 codes in three words (bits 6k of 96). Adding +0 in the scaling makes a -0
-// product +0 (to_e2m3x2's other replacement, NaN, is only made where max_abs16 saw one), and four codes in
-// four bytes become 24 bits with two byte dot products (weights 1 and 64) and a multiply-add.
+// 16 values times `inv`, as 16 codes in three words (bits 6k of 96). Adding +0 to the rounded product makes a -0 product
+// +0 (to_e2m3x2's other replacement, NaN, is only made where max_abs16 saw one). The multiply-add alone would not: a
+// negative product too small for FP32, as of -1e-30 beside 1e24, is not zero before its rounding, which then gives -0. The
+// product is a multiply-add because a packed multiplication and the packed addition after it were joined into one: the
+// bytes showed it. Four codes in four bytes become 24 bits with two byte dot products (weights 1 and 64) and a multiply-add.
 __device__ __forceinline__ void quantize16(const float* v, float inv, bool nan, uint32_t& w0, uint32_t& w1,
                                            uint32_t& w2) {
     uint32_t q[8], g[4];  // q[i] = code(v[2i]) | code(v[2i + 1]) << 8
@@ -113,7 +115,7 @@ __device__ __forceinline__ void quantize16(const float* v, float inv, bool nan, 
         for (int i = 0; i < 8; i++) {
             uint16_t d;
             float lo, hi;
-            split(fma(pair(v[2 * i], v[2 * i + 1]), both(inv), both(0.0f)), lo, hi);
+            split(fma(pair(v[2 * i], v[2 * i + 1]), both(inv), both(0.0f)) + both(0.0f), lo, hi);
             asm("cvt.rn.satfinite.e2m3x2.f32 %0, %1, %2;" : "=h"(d) : "f"(hi), "f"(lo));
             q[i] = d;
         }

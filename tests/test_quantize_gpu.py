@@ -145,3 +145,55 @@ def test_activation_path_on_device(lib, oracle, M, N, K):
     sA_pad = lib.pad_scales_k(host.scales, M, K)
     assert np.array_equal(a_packed.cpu().numpy(), A_pad)
     check(D.cpu(), oracle.gemm(A_pad, sA_pad, b.Bt, b.sB, Kp), lib.OutType.F32, oracle, label=f"ffn {M}x{N}x{K}")
+
+
+def _wide_range_blocks(rows, cols, seed, dtype=torch.float32):
+    """Values from subnormal to huge in one block, both signs; NaN in some half blocks."""
+    rng = np.random.default_rng(seed)
+    top = rng.uniform(-10, 38, (rows, cols // 32, 1))
+    exp = rng.uniform(-45, np.broadcast_to(top, (rows, cols // 32, 32)))
+    exp[:, :, 5] = top[:, :, 0]
+    m = 10.0 ** exp * rng.choice([-1.0, 1.0], exp.shape)
+    m[0, 0, :4], m[0, -1, :4] = [1e24, -1e-30, 1e-30, -1e-38], [1e6, -1e-42, -1e-20, 1e-42]
+    m[rng.random(exp.shape[:2]) < 0.2, 20] = np.nan
+    return torch.from_numpy(m.reshape(rows, cols).astype(np.float32)).to(dtype)
+
+
+@pytest.mark.parametrize("tiled", [False, True])
+def test_tiny_values_beside_large_ones(lib, tiled):
+    """A negative value far below its block's scale: the scaled value underflows to -0, whose code is 0."""
+    rows, cols = 300, 1024
+    m = _wide_range_blocks(rows, cols, 5)
+    host = lib.quantize_to_mxfp6(m.numpy())
+    p, s = _device_quantize(lib, m.numpy(), tiled)
+    assert np.array_equal(p, host.packed_data)
+    assert np.array_equal(lib.untile_scales(s, rows, cols) if tiled else s.reshape(rows, -1), host.scales)
+    for ot, dtype in ((lib.OutType.F32, torch.float32), (lib.OutType.BF16, torch.bfloat16)):
+        x = _wide_range_blocks(rows, cols, 6, dtype)
+        host = lib.quantize_to_mxfp6(x.float().numpy())
+        packed = torch.empty(rows, cols * 3 // 4, dtype=torch.uint8, device="cuda")
+        scales = torch.empty(rows, cols // 32, dtype=torch.uint8, device="cuda")
+        assert lib.quantize_device_typed(x.cuda(), ot, rows, cols, cols, cols, packed, scales) == lib.OK
+        torch.cuda.synchronize()
+        assert np.array_equal(packed.cpu().numpy(), host.packed_data) and np.array_equal(scales.cpu().numpy(), host.scales)
+
+
+# few rows over a cluster, one tile, split K with its reduce, the pair
+@pytest.mark.parametrize("M,N,K", [(1, 512, 256), (5, 512, 2048), (300, 512, 256), (200, 2048, 4096), (2050, 6144, 256)])
+def test_fused_output_has_the_quantisers_bytes(lib, M, N, K):
+    """Zero operands, so that the fused GEMM's values are its bias: its MXFP6 rows are the host quantiser's on every route."""
+    Kp, rb = K, K * 3 // 4
+    A, B = (torch.zeros(r, rb, dtype=torch.uint8, device="cuda") for r in (M, N))
+    sA, sB = (torch.full((lib.tiled_scale_bytes(r, K),), 127, dtype=torch.uint8, device="cuda") for r in (M, N))
+    bias = _wide_range_blocks(1, N, 7 + M)
+    host = lib.quantize_to_mxfp6(bias.numpy())
+    packed = torch.empty(M, N * 3 // 4, dtype=torch.uint8, device="cuda")
+    scales = torch.empty(lib.tiled_scale_bytes(M, N), dtype=torch.uint8, device="cuda")
+    n = lib.gemm_fused_workspace_size(M, N, Kp)
+    ws = torch.empty(n, dtype=torch.uint8, device="cuda") if n else None
+    ep = lib.Epilogue(bias=bias.view(-1).cuda(), bias_type=lib.OutType.F32)
+    assert lib.gemm_fused_quant(M, N, Kp, A, B, sA, sB, packed, scales, rb, rb, ep, ws, n) == lib.OK
+    torch.cuda.synchronize()
+    assert lib.device_status() == 0
+    assert np.array_equal(packed.cpu().numpy(), np.repeat(host.packed_data, M, 0))
+    assert np.array_equal(lib.untile_scales(scales.cpu().numpy(), M, N), np.repeat(host.scales, M, 0))
