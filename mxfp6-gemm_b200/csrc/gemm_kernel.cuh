@@ -533,9 +533,9 @@ __global__ void __launch_bounds__(Config<BN, AMODE, FusedTraits<OutT>::fused, Fu
 
 // Split-K second stage (reference: src/kernel.hpp:305-313): D = sum_{s=0..S-1} ws[s], in that
 // fixed order, converted once and written to every destination of the list. Four elements per
-// thread per step (N % 4 == 0, so the four stay in one row).
+// thread per step (N % 4 == 0, so the four stay in one row). `ws` is not __restrict__: it is written until griddep_wait.
 template <typename OutT>
-__global__ void __launch_bounds__(256) reduce_partials(const float* __restrict__ ws, const DstList dl, int N,
+__global__ void __launch_bounds__(256) reduce_partials(const float* ws, const DstList dl, int N,
                                                        long long total, int S) {
     sm100::griddep_launch_dependents();
     sm100::griddep_wait();  // the partials of the GEMM before it
@@ -573,7 +573,7 @@ __global__ void __launch_bounds__(256) reduce_partials(const float* __restrict__
 // The partials have a pitch of Np columns (N rounded up to 32). A thread takes four columns; the
 // eight threads of a 32-column block are consecutive lanes of one warp (blocks never straddle: Np is
 // a multiple of 32), so MXFP6 output takes the block's maximum over three shuffles.
-__global__ void __launch_bounds__(256) reduce_partials_fused(const float* __restrict__ ws, const Epi e, int M, int N,
+__global__ void __launch_bounds__(256) reduce_partials_fused(const float* ws, const Epi e, int M, int N,
                                                              int Np, int S) {
     sm100::griddep_launch_dependents();
     sm100::griddep_wait();  // the partials of the GEMM before it

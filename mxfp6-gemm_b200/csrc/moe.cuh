@@ -525,12 +525,12 @@ __global__ void __launch_bounds__(ProductConfig<KIND, NMAX>::THREADS, ProductCon
     if (!EARLY) sm100::griddep_wait();
     // An entry, past L1: its lines are only sure to be newer than the list after the wait.
     auto entry = [&](int a) {
-        const int4 q = __ldcg(reinterpret_cast<const int4*>(p.entries) + a);
+        const int4 q = sm100::ld_l2_s32x4(reinterpret_cast<const int4*>(p.entries) + a);
         return Entry{q.x, q.y, q.z, q.w};
     };
     // the first item's entry is read beside the count (it exists in the workspace whatever the count is)
     const Entry first = entry((int)blockIdx.x / p.tiles);
-    const int total = __ldcg(p.n_entries) * p.tiles;
+    const int total = sm100::ld_l2_s32(p.n_entries) * p.tiles;
     if (EARLY && warp != 0) sm100::griddep_wait();
     if (!EARLY || warp != 0) sm100::griddep_launch_dependents();
     // the entry of item `it`, read an item ahead of its use
@@ -816,8 +816,8 @@ __global__ void __launch_bounds__(256) moe_combine(const CombineParams p) {
     // the places and weights were complete when the down product let this kernel start (see moe_product): read them
     // before the wait, past L1
     const int t = blockIdx.y, col = (blockIdx.x * blockDim.x + threadIdx.x) * 4, lane = threadIdx.x & 31;
-    const int slot = lane < p.top_k ? __ldcg(p.slot_of + t * p.top_k + lane) : -1;
-    const float weight = lane < p.top_k ? __ldcg(p.slot_w + t * p.top_k + lane) : 0.0f;
+    const int slot = lane < p.top_k ? sm100::ld_l2_s32(p.slot_of + t * p.top_k + lane) : -1;
+    const float weight = lane < p.top_k ? sm100::ld_l2_f32(p.slot_w + t * p.top_k + lane) : 0.0f;
     sm100::griddep_wait();
     float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     const bool in = col < p.hidden;

@@ -197,3 +197,37 @@ def test_fused_output_has_the_quantisers_bytes(lib, M, N, K):
     assert lib.device_status() == 0
     assert np.array_equal(packed.cpu().numpy(), np.repeat(host.packed_data, M, 0))
     assert np.array_equal(lib.untile_scales(scales.cpu().numpy(), M, N), np.repeat(host.scales, M, 0))
+
+
+@pytest.mark.parametrize("M,N,K", [(40, 2048, 1024), (700, 4096, 512), (200, 2048, 4096)])
+def test_typed_quantiser_reads_what_the_kernel_before_wrote(lib, M, N, K):
+    """The quantiser starts while the fused GEMM before it still writes the rows it reads: other values in the same buffer
+    at every step, none of them an earlier step's."""
+    rb = K * 3 // 4
+    rng = np.random.default_rng(M)
+    A, B = (lib.quantize_to_mxfp6(rng.standard_normal((r, K), dtype=np.float32)) for r in (M, N))
+    a, b = torch.from_numpy(A.packed_data).cuda(), torch.from_numpy(B.packed_data).cuda()
+    sa, sb = (torch.from_numpy(lib.preprocess_scale(q.scales, r, K)).cuda() for q, r in ((A, M), (B, N)))
+    n = lib.gemm_fused_workspace_size(M, N, K)
+    ws = torch.empty(n, dtype=torch.uint8, device="cuda") if n else None
+    steps = 12
+    biases = [torch.randn(N, generator=torch.Generator().manual_seed(i)).mul_(64).cuda() for i in range(steps)]
+    eps = [lib.Epilogue(bias=x, bias_type=lib.OutType.F32) for x in biases]
+    y = torch.zeros(M, N, dtype=torch.bfloat16, device="cuda")
+    kept = [torch.empty_like(y) for _ in range(steps)]
+    packed = [torch.empty(M, N * 3 // 4, dtype=torch.uint8, device="cuda") for _ in range(steps)]
+    scales = [torch.empty(M, N // 32, dtype=torch.uint8, device="cuda") for _ in range(steps)]
+
+    def gemm(i, out):
+        assert lib.gemm_fused(lib.OutType.BF16, M, N, K, a, b, sa, sb, out, rb, rb, eps[i], ws, n) == lib.OK
+
+    for i in range(steps):
+        gemm(i, kept[i])
+    torch.cuda.synchronize()
+    for i in range(steps):
+        gemm(i, y)
+        assert lib.quantize_device_typed(y, lib.OutType.BF16, M, N, N, N, packed[i], scales[i]) == lib.OK
+    torch.cuda.synchronize()
+    for i in range(steps):
+        want = lib.quantize_to_mxfp6(kept[i].float().cpu().numpy())
+        assert np.array_equal(packed[i].cpu().numpy(), want.packed_data) and np.array_equal(scales[i].cpu().numpy(), want.scales)
