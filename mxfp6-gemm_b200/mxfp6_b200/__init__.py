@@ -262,30 +262,107 @@ def gemm_gather(ot, M, N, Kp, dA, dBsh, dsA, dsB, dDs, ldd, col0, A_row_bytes, B
             A_row_bytes, B_row_bytes, _addr(ws), ws_bytes, s)
 
 
+# Element type of a tensor -> its OutType (None for whole numbers, which stand for raw memory), and its name.
+_KINDS: dict = {}
+_NAMES: dict = {}
+
+
+def _kind_of(t):
+    """OutType of a tensor's elements; None for an address or raw memory."""
+    if t is None or isinstance(t, int):
+        return None
+    try:
+        return _KINDS[t.dtype]
+    except AttributeError:
+        return None
+    except KeyError:
+        name = str(t.dtype).rpartition(".")[2]
+        kind = {"float32": OutType.F32, "float16": OutType.F16, "bfloat16": OutType.BF16}.get(name)
+        if kind is None and ("float" in name or "complex" in name):
+            raise ValueError(f"elements of {t.dtype}: the library reads and writes float32, float16 and bfloat16") from None
+        _KINDS[t.dtype] = kind
+        return kind
+
+
+def _check_kind(what, t, kind):
+    have = _kind_of(t)
+    if have is not None and have != kind:
+        raise ValueError(f"{what} has elements of {t.dtype}, the call says {kind!r}")
+
+
+def _check_dense(what, t, name):
+    """A tensor (or None, or an address) that the library takes as dense elements of the type `name`."""
+    dtype = getattr(t, "dtype", None)
+    if dtype is None:
+        return
+    if _NAMES.get(dtype) != name and str(dtype).rpartition(".")[2] != name:
+        raise ValueError(f"{what} has elements of {dtype}, not {name}")
+    if not t.is_contiguous():
+        raise ValueError(f"{what} is not contiguous")
+    _NAMES[dtype] = name
+
+
+def _columns(what, t) -> bool:
+    """Whether t is a tensor with strides; its columns have to lie next to one another."""
+    if not hasattr(t, "stride") or not t.dim():
+        return False
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
+        raise ValueError(f"{what} has a column stride of {t.stride(-1)}: columns have to lie next to one another")
+    return True
+
+
+def _pitch(what, t, ld, cols) -> int:
+    """Elements between rows of `cols` elements: `ld` where it is given, else `cols` for an address or a contiguous tensor
+    and the row stride of any other [rows][cols] tensor."""
+    if t is None or isinstance(t, int):
+        return cols if ld is None else ld
+    try:
+        if t.is_contiguous():
+            return cols if ld is None else ld
+    except AttributeError:  # an object with an address alone
+        return cols if ld is None else ld
+    _columns(what, t)
+    if ld is not None:
+        return ld
+    if t.dim() == 2 and t.shape[1] == cols:
+        return t.stride(0)
+    raise ValueError(f"{what}: the row stride is needed for a tensor that is neither [rows][{cols}] nor contiguous")
+
+
 class Epilogue:
     """The epilogue of gemm_fused / gemm_fused_quant (struct mxfp6_epilogue): op(act(A·B + bias), aux).
-    bias: N elements of bias_type; aux: [M][ld_aux] of aux_type (ld_aux may be left out for a tensor,
-    whose row stride it then is). Build it once and pass it to any number of calls; it keeps the
-    operands it was given alive."""
+    bias: N elements of bias_type; aux: [M][ld_aux] of aux_type. The types and ld_aux may be left out for tensors, whose
+    element type and row stride they then are (F32 for addresses). A tensor of another type than the one given, a bias
+    that is not contiguous and an aux whose columns are apart raise ValueError. Build it once and pass it to any number of
+    calls; it keeps the operands it was given alive."""
 
-    def __init__(self, bias=None, bias_type=OutType.F32, act=Act.NONE, aux=None, aux_type=OutType.F32,
-                 aux_op=AuxOp.NONE, ld_aux=None):
+    def __init__(self, bias=None, bias_type=None, act=Act.NONE, aux=None, aux_type=None, aux_op=AuxOp.NONE, ld_aux=None):
+        kinds = []
+        for what, t, kind in (("bias", bias, bias_type), ("aux", aux, aux_type)):
+            have = _kind_of(t)
+            kind = have if kind is None else kind
+            kinds.append(OutType.F32 if kind is None else kind)
+            _check_kind(what, t, kinds[-1])
+        if hasattr(bias, "is_contiguous") and not bias.is_contiguous():
+            raise ValueError("bias is not contiguous")
+        rows = _columns("aux", aux) and aux.dim() > 1 and aux.shape[0] > 1
         if ld_aux is None:
             if isinstance(aux, int):
                 raise ValueError("ld_aux is needed for an aux operand given as an address")
-            ld_aux = 0 if aux is None else aux.stride(0)
+            ld_aux = 0 if aux is None else aux.stride(0) if rows else aux.shape[-1]
         self.keep = (bias, aux)
-        self.struct = _EpilogueStruct(_addr(bias), _addr(aux), ld_aux, int(bias_type), int(act), int(aux_op),
-                                      int(aux_type))
+        self.struct = _EpilogueStruct(_addr(bias), _addr(aux), ld_aux, int(kinds[0]), int(act), int(aux_op), int(kinds[1]))
         self.ref = C.addressof(self.struct)
 
 
 def gemm_fused(ot, M, N, Kp, dA, dBsh, dsA, dsB, dD, A_row_bytes, B_row_bytes, epilogue=None, ws=None, ws_bytes=0,
                stream=None, ldd=None) -> int:
     """mxfp6_gemm_fused: D = op(act(A·B + bias), aux) for any M >= 0 and N > 0, rows of D ldd
-    elements apart (N by default). Asynchronous; returns an mxfp6_status."""
+    elements apart (by default the row stride of an [M][N] tensor, else N). A tensor D of another type than ot raises
+    ValueError. Asynchronous; returns an mxfp6_status."""
+    _check_kind("D", dD, ot)
     return _gemm_fused(int(ot), M, N, Kp, _addr(dA), _addr(dBsh), _addr(dsA), _addr(dsB), _addr(dD),
-                       N if ldd is None else ldd, A_row_bytes, B_row_bytes, epilogue.ref if epilogue else 0,
+                       _pitch("D", dD, ldd, N), A_row_bytes, B_row_bytes, epilogue.ref if epilogue else 0,
                        _addr(ws), ws_bytes, _stream_arg(stream))
 
 
@@ -323,12 +400,19 @@ def moe_workspace_size(layer: MoELayer, tokens: int, top_k: int) -> int:
 def moe(layer, ot, tokens, top_k, x, x_type, out, ws, ws_bytes, logits=None, renormalize=True, ids=None, weights=None,
         residual=None, ldx=None, ldo=None, ld_residual=None, stream=None) -> int:
     """mxfp6_moe: a mixture-of-experts layer for up to 128 tokens, routed by logits (ids and weights then
-    receive the choice) or by the given ids and weights. Row strides default to layer.hidden.
-    Asynchronous; returns an mxfp6_status."""
+    receive the choice) or by the given ids and weights. Row strides default to those of [tokens][layer.hidden] tensors,
+    else to layer.hidden. Tensors of other types than x_type and ot, logits and weights that are not dense float32, and ids
+    that are not dense int32 raise ValueError. Asynchronous; returns an mxfp6_status."""
     H = layer.hidden
-    return _moe(layer.ref, int(ot), tokens, top_k, _addr(x), int(x_type), H if ldx is None else ldx, _addr(logits),
-                int(renormalize), _addr(ids), _addr(weights), _addr(residual), H if ld_residual is None else ld_residual,
-                _addr(out), H if ldo is None else ldo, _addr(ws), ws_bytes, _stream_arg(stream))
+    _check_kind("x", x, x_type)
+    _check_kind("out", out, ot)
+    _check_kind("residual", residual, ot)
+    _check_dense("logits", logits, "float32")
+    _check_dense("ids", ids, "int32")
+    _check_dense("weights", weights, "float32")
+    return _moe(layer.ref, int(ot), tokens, top_k, _addr(x), int(x_type), _pitch("x", x, ldx, H), _addr(logits),
+                int(renormalize), _addr(ids), _addr(weights), _addr(residual), _pitch("residual", residual, ld_residual, H),
+                _addr(out), _pitch("out", out, ldo, H), _addr(ws), ws_bytes, _stream_arg(stream))
 
 
 def ipc_export(t) -> tuple[bytes, int]:
@@ -416,7 +500,10 @@ def quantize_device_padded(d_mat, rows, cols, padded_cols, d_packed, d_scales, t
 def quantize_device_typed(d_mat, in_type, rows, cols, ld, padded_cols, d_packed, d_scales, tiled=False,
                           stream=None) -> int:
     """mxfp6_quantize_device_typed: rows of F32 / F16 / BF16 values, ld elements apart, quantised to
-    rows of padded_cols codes (device pointers). Returns an mxfp6_status."""
+    rows of padded_cols codes (device pointers). A tensor of another type than in_type, or with its columns apart, raises
+    ValueError. Returns an mxfp6_status."""
+    _check_kind("d_mat", d_mat, in_type)
+    _pitch("d_mat", d_mat, ld, cols)
     return _quantize_dev_t(_addr(d_mat), int(in_type), rows, cols, ld, padded_cols, _addr(d_packed), _addr(d_scales),
                            1 if tiled else 0, _stream_arg(stream))
 

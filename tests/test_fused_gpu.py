@@ -407,3 +407,17 @@ def test_compact_a_in_place_repeats(M, N, K):
             assert all(torch.equal(D, first) for D in outs)
     finally:
         lib.set_repad_scratch(prev)
+
+
+def test_types_and_strides_of_tensors():
+    """Operands given as tensors alone: their element types and row strides are the call's."""
+    M, N, K = 33, 200, 256
+    A, B = Operand(M, K, 1.0, 70), Operand(N, K, 0.06, 71)
+    bias, aux = _randn(N, seed=72, dtype=torch.bfloat16), _randn(M, N + 16, seed=73, dtype=torch.float16)[:, 8:N + 8]
+    D = torch.full((M, N + 8), 7.0, dtype=torch.bfloat16, device="cuda")
+    ep = lib.Epilogue(bias, act=Act.SILU, aux=aux, aux_op=AuxOp.MUL)
+    assert lib.gemm_fused(OutType.BF16, M, N, A.Kp, A.packed, B.packed, A.scales, B.scales, D[:, :N], A.row_bytes,
+                          B.row_bytes, ep) == lib.OK
+    _finish()
+    assert (D[:, N:] == 7.0).all()
+    check_rounded(D[:, :N], *fused64(A, B, Act.SILU, bias, aux, AuxOp.MUL), OutType.BF16)

@@ -79,3 +79,63 @@ def test_workspace_query(lib):
 def test_aux_given_as_an_address_needs_its_pitch(lib):
     with pytest.raises(ValueError):
         lib.Epilogue(aux=P, aux_op=lib.AuxOp.ADD)
+
+
+@pytest.fixture
+def torch():
+    return pytest.importorskip("torch")
+
+
+@pytest.fixture
+def seen(lib, monkeypatch):
+    """The arguments of the C calls, which are not made."""
+    got = []
+    for name in ("_gemm_fused", "_quantize_dev_t"):
+        monkeypatch.setattr(lib, name, lambda *a: got.append(a) or 0)
+    return got
+
+
+@pytest.mark.parametrize("dtype,kind", [("float32", "F32"), ("float16", "F16"), ("bfloat16", "BF16")])
+def test_epilogue_takes_a_tensors_type_and_stride(lib, torch, dtype, kind):
+    t = getattr(torch, dtype)
+    bias, aux = torch.zeros(40, dtype=t), torch.zeros(5, 56, dtype=t)[:, 8:48]
+    want = int(lib.OutType[kind])
+    for e in (lib.Epilogue(bias, aux=aux, aux_op=lib.AuxOp.ADD),
+              lib.Epilogue(bias, want, aux=aux, aux_type=want, aux_op=lib.AuxOp.ADD)):
+        s = e.struct
+        assert (s.bias, s.bias_type, s.aux, s.aux_type, s.ld_aux) == (bias.data_ptr(), want, aux.data_ptr(), want, 56)
+    assert lib.Epilogue(aux=aux[:1]).struct.ld_aux >= 40 and lib.Epilogue(aux=aux[0]).struct.ld_aux == 40
+    assert lib.Epilogue(bias=P, aux=P, ld_aux=40).struct.bias_type == lib.OutType.F32
+    for other in set(lib.OutType) - {want}:
+        for kw in (dict(bias=bias, bias_type=other), dict(aux=aux, aux_type=other)):
+            with pytest.raises(ValueError, match="elements"):
+                lib.Epilogue(**kw)
+
+
+def test_epilogue_refuses_what_it_would_read_wrongly(lib, torch):
+    for kw in (dict(bias=torch.zeros(40, dtype=torch.float64)), dict(aux=torch.zeros(5, 40, dtype=torch.float64)),
+               dict(bias=torch.zeros(80)[::2]), dict(aux=torch.zeros(40, 5).T), dict(aux=torch.zeros(5, 80)[:, ::2], ld_aux=80)):
+        with pytest.raises(ValueError):
+            lib.Epilogue(**kw)
+
+
+def test_fused_output_tensor(lib, torch, call, seen):
+    D = torch.zeros(5, 64, dtype=torch.float16)[:, :40]
+    for kw, ldd in ((dict(D=D), 64), (dict(D=D, ldd=70), 70), (dict(D=D[:1].contiguous(), M=1), 40), (dict(D=P), 40),
+                    (dict(D=torch.zeros(200, dtype=torch.uint8)), 40)):
+        assert call(**kw) == 0 and seen[-1][9] == ldd
+    n = len(seen)
+    for kw in (dict(D=D, ot=lib.OutType.F32), dict(D=D.double()), dict(D=torch.zeros(40, 5, dtype=torch.float16).T),
+               dict(D=torch.zeros(4, 5, 40, dtype=torch.float16)[::2])):
+        with pytest.raises(ValueError):
+            call(**kw)
+    assert len(seen) == n
+
+
+def test_typed_quantiser_input_tensor(lib, torch, seen):
+    x = torch.zeros(4, 64, dtype=torch.bfloat16)
+    assert lib.quantize_device_typed(x, lib.OutType.BF16, 4, 64, 64, 64, P, P) == 0
+    for bad, t in ((x, lib.OutType.F32), (x.T, lib.OutType.BF16), (x.double(), lib.OutType.F32)):
+        with pytest.raises(ValueError):
+            lib.quantize_device_typed(bad, t, 4, 64, 64, 64, P, P)
+    assert len(seen) == 1

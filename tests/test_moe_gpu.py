@@ -349,3 +349,18 @@ def test_weight_scales_of_every_slab(T, k, E):
         torch.cuda.synchronize()
         assert all(torch.equal(out, first) for out in outs)
     assert lib.device_status() == 0
+
+
+def test_strides_of_tensors():
+    """x, out and residual as views of wider rows, their strides taken from the tensors."""
+    layer, T, k, ot = Layer(4, 256, 128), 5, 2, OutType.BF16
+    x = _randn(T, 272, seed=130, dtype=torch.bfloat16)[:, 8:264]
+    res = _randn(T, 300, seed=131, dtype=torch.bfloat16)[:, :256]
+    buf = torch.full((T, 261), 9.0, dtype=torch.bfloat16, device="cuda")
+    ids = torch.tensor([[0, 1], [1, 2], [2, 3], [3, 0], [1, 3]], dtype=torch.int32, device="cuda")
+    w = _randn(T, k, seed=132)
+    ws, n = _space(layer, T, k)
+    assert lib.moe(layer.layer, ot, T, k, x, ot, buf[:, :256], ws, n, ids=ids, weights=w, residual=res) == lib.OK
+    torch.cuda.synchronize()
+    assert lib.device_status() == 0 and (buf[:, 256:] == 9.0).all()
+    check_rounded(buf[:, :256], *layer.reference(x, ids, w, res), ot)

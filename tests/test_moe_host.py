@@ -46,3 +46,29 @@ def test_workspace_query(lib):
     sizes = [lib.moe_workspace_size(layer, t, 2) for t in range(1, 129)]
     # quantised rows, hidden rows and FP32 rows for every choice
     assert all(n >= 2 * t * (256 + 128 + 4 * 256) for t, n in enumerate(sizes, 1))
+
+
+def test_tensors_types_and_strides(lib, monkeypatch):
+    torch = pytest.importorskip("torch")
+    seen = []
+    monkeypatch.setattr(lib, "_moe", lambda *a: seen.append(a) or 0)
+    layer, F16, BF16 = _layer(lib), lib.OutType.F16, lib.OutType.BF16
+    x = torch.zeros(4, 300, dtype=torch.bfloat16)[:, 1:257]
+    out, res = torch.zeros(4, 261, dtype=torch.float16)[:, :256], torch.zeros(4, 260, dtype=torch.float16)[:, :256]
+    good = dict(ot=F16, x=x, x_type=BF16, out=out, residual=res, logits=torch.zeros(4, 8),
+                ids=torch.zeros(4, 2, dtype=torch.int32), weights=torch.zeros(4, 2))
+    pitches = lambda a: (a[6], a[12], a[14])  # noqa: E731
+    assert _call(lib, layer, **good) == 0 and pitches(seen[-1]) == (300, 260, 261)
+    assert _call(lib, layer, **good | dict(ldx=301, ldo=302, ld_residual=303)) == 0 and pitches(seen[-1]) == (301, 303, 302)
+    dense = dict(x=x.reshape(2, 512), out=torch.zeros(1024, dtype=torch.float16), residual=None)
+    assert _call(lib, layer, **good | dense) == 0 and pitches(seen[-1]) == (256, 256, 256)
+    assert _call(lib, layer, **good | dict(tokens=1, x=x[:1], out=P, residual=P)) == 0 and pitches(seen[-1]) == (256, 256, 256)
+    n = len(seen)
+    for bad in (dict(x_type=F16), dict(ot=BF16), dict(residual=res.float()), dict(out=out.double()),
+                dict(x=torch.zeros(256, 4, dtype=torch.bfloat16).T), dict(out=torch.zeros(8, 261, dtype=torch.float16)[:, :200]),
+                dict(logits=torch.zeros(4, 8, dtype=torch.bfloat16)), dict(logits=torch.zeros(4, 16)[:, :8]),
+                dict(ids=torch.zeros(4, 2, dtype=torch.int64)), dict(ids=torch.zeros(2, 4, dtype=torch.int32).T),
+                dict(weights=torch.zeros(4, 2, dtype=torch.float16))):
+        with pytest.raises(ValueError):
+            _call(lib, layer, **good | bad)
+    assert len(seen) == n
