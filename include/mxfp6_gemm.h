@@ -102,7 +102,9 @@ void mxfp6_gemm_gather(int ot, int M, int N, int Kp, const void* dA, const void*
  * further kernels. */
 
 /* Activations: v, max(v, 0), v*Phi(v) with the error function, its tanh form
- * 0.5 v (1 + tanh(sqrt(2/pi) (v + 0.044715 v^3))), and v / (1 + e^-v). */
+ * 0.5 v (1 + tanh(sqrt(2/pi) (v + 0.044715 v^3))), and v / (1 + e^-v). Relative errors, before the output's rounding:
+ * GELU 2^-19 + 2^-23 v^2 (0 from v = -13.3 down), its tanh form 2^-20 + 2^-21 |v| (1 + 0.0447 v^2), SiLU 2^-20 + 2^-23 |v|;
+ * the tanh form below -7.5 and SiLU below -43 stay at the value there, -4e-18 and -9e-18. */
 enum mxfp6_activation {
     MXFP6_ACT_NONE = 0, MXFP6_ACT_RELU = 1, MXFP6_ACT_GELU = 2, MXFP6_ACT_GELU_TANH = 3, MXFP6_ACT_SILU = 4
 };

@@ -78,26 +78,34 @@ __device__ __forceinline__ F2 over_one_plus_ex2(F2 v, F2 y) {
     return v * rcp<true>(fminf(a, 0x1p63f), fminf(b, 0x1p63f));  // a NaN must not reach the other value
 }
 
-// v Phi(v) = max(v, 0) - |v| erfc(|v| / sqrt(2)) / 2, with erfc(x) = (a1 t + ... + a5 t^5) e^(-x^2), t = 1 / (1 + p x)
-// (Hastings; Abramowitz and Stegun 7.1.26: absolute error 1.5e-7; the coefficients here are halved, and
-// e^(-x^2) = 2^(-v^2 log2(e) / 2)). From |v| = 16 on the second term is 0 in FP32.
+// v Phi(v) = max(v, 0) - |v| erfc(|v| / sqrt(2)) / 2, and erfc(u / sqrt(2)) / 2 = (a1 t + ... + a8 t^8) e^(-u^2 / 2),
+// t = 1 / (1 + p u). The polynomial is a fit of this header's own: the quotient of the two sides is within 7.8e-8 of 1 for
+// u in [0, 13.3] (least largest relative error, at this p), so that the negative tail keeps its digits, which a form with an
+// absolute bound does not (with the five coefficients of Abramowitz and Stegun 7.1.26 it was 2e-3 off at -5, 1e-2 at -8).
+// e^(-u^2 / 2) = 2^(-u^2 log2(e) / 2) adds its argument's rounding, 2^-23 u^2; from u = 13.3 on it is 0. In all the relative
+// error is below 2^-19 + 2^-23 v^2: t is off by 5 half steps at most, which count 3.4 times at u = 0.
 template <bool SHARE>
 __device__ __forceinline__ F2 gelu_erf(float v0, float v1) {
     const float u0 = fminf(fabsf(v0), 16.0f), u1 = fminf(fabsf(v1), 16.0f);
     const F2 u = pair(u0, u1);
     float a, b;
-    split(fma(u, both(0.3275911f * 0.70710678118654752f), both(1.0f)), a, b);
+    split(fma(u, both(0.233f), both(1.0f)), a, b);
     const F2 t = rcp<SHARE>(a, b);
-    F2 q = fma(t, both(0.5f * 1.061405429f), both(0.5f * -1.453152027f));
-    q = fma(q, t, both(0.5f * 1.421413741f));
-    q = fma(q, t, both(0.5f * -0.284496736f));
-    q = fma(q, t, both(0.5f * 0.254829592f));
+    F2 q = fma(t, both(-0.0687599108f), both(0.235863566f));
+    q = fma(q, t, both(-0.184671089f));
+    q = fma(q, t, both(0.212113991f));
+    q = fma(q, t, both(0.0195844453f));
+    q = fma(q, t, both(0.101660840f));
+    q = fma(q, t, both(0.0911546126f));
+    q = fma(q, t, both(0.0930535197f));
     const F2 half_erfc = q * t * ex2(u * u * both(-0.5f * LOG2E));
     return fma(pair(-u0, -u1), half_erfc, pair(max_nan(v0, 0.0f), max_nan(v1, 0.0f)));
 }
 
-// The quotients have no cancellation anywhere, so they stay within a few FP32 ulp. Below -43 (-7.5) SiLU (the tanh form of
-// GELU) is the value there, -9e-18 (-4e-18), instead of one even nearer to 0: 1 + e^43 is what the shared reciprocal takes.
+// The quotients have no cancellation anywhere: a few FP32 ulp, and on the negative side the rounding of the exponent, 2^-23 |v|
+// for SiLU (2^-20 + 2^-23 |v| in all) and 2^-21 |v| (1 + 0.0447 v^2) for the tanh form of GELU (2^-20 more in all). Below -43
+// (-7.5) SiLU (the tanh form) is the value there, -9e-18 (-4e-18), instead of one even nearer to 0: 1 + e^43 is what the
+// shared reciprocal takes.
 template <int ACT, bool SHARE>
 __device__ __forceinline__ F2 activate(float v0, float v1) {
     if constexpr (ACT == ACT_RELU) return pair(max_nan(v0, 0.0f), max_nan(v1, 0.0f));

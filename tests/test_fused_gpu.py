@@ -421,3 +421,30 @@ def test_types_and_strides_of_tensors():
     _finish()
     assert (D[:, N:] == 7.0).all()
     check_rounded(D[:, :N], *fused64(A, B, Act.SILU, bias, aux, AuxOp.MUL), OutType.BF16)
+
+
+def _activation_bound(act, v):
+    """Relative error of an activation on FP32 values: roundings of the exponent, which grow with its size, and 2^-20 or
+    2^-19 for the reciprocal (with a shared one t is off by five half steps), the exponential (two ulp) and the rest."""
+    if act == Act.GELU:
+        return 2.0 ** -19 + 2.0 ** -23 * v ** 2
+    return 2.0 ** -20 + (2.0 ** -23 * v.abs() if act == Act.SILU else 2.0 ** -21 * v.abs() * (1 + 0.0447 * v ** 2))
+
+
+# one row, few rows by columns and in fours, one tile in both layouts, split K, the pair
+@pytest.mark.parametrize("M,N,K", [(1, 4096, 128), (3, 4095, 128), (40, 4095, 128), (40, 4096, 128), (300, 4096, 128),
+                                   (300, 4095, 128), (200, 2048, 4096), (2050, 6144, 128)])
+@pytest.mark.parametrize("act,low", [(Act.GELU, -12.9), (Act.GELU_TANH, -7.5), (Act.SILU, -43.0)])
+def test_activations_relative_error(M, N, K, act, low):
+    """Zero operands: the activation of the bias alone, relative to its value, down to where it ends."""
+    A, B = Operand(M, K, 0.0, 80), Operand(N, K, 0.0, 81)
+    rng = np.random.default_rng(82)
+    for v in (rng.uniform(low, 6.0, N), rng.uniform(-3.0, 3.0, N), rng.choice([-1.0, 1.0], N) * 10.0 ** rng.uniform(-30, 0.4, N)):
+        v = torch.from_numpy(v.astype(np.float32)).cuda()
+        got, x = _fused(A, B, OutType.F32, act, v), v.double()
+        assert (got == got[0]).all()
+        ref = x * torch.special.erfc(-x * np.sqrt(0.5)) / 2 if act == Act.GELU else x * torch.sigmoid(
+            x if act == Act.SILU else 2 * np.sqrt(2 / np.pi) * (x + 0.044715 * x ** 3))
+        off = (got[0].double() / ref - 1).abs()
+        worst = (off - _activation_bound(act, x)).argmax()
+        assert (off <= _activation_bound(act, x)).all(), (act, float(x[worst]), float(off[worst]))
