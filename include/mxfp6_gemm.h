@@ -154,7 +154,8 @@ size_t mxfp6_gemm_fused_workspace_size(int M, int N, int Kp, int A_row_bytes);
  *   e = ids[t][j]; without a gate h = act(up_e(x[t]))
  *
  * As everywhere in this library both operands of each product are MXFP6: x and h are quantised as by
- * mxfp6_quantize_device, sums are FP32, and out is rounded once. */
+ * mxfp6_quantize_device, sums are FP32 (an FP32 output's of more than 12288 products in segments, as mxfp6_gemm's), and out
+ * is rounded once. */
 typedef struct mxfp6_moe_layer {
     int experts;            /* 1..512 */
     int hidden, inter;      /* multiples of 128 */

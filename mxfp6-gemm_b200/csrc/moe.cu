@@ -6,6 +6,7 @@
 
 #include "host.hpp"
 #include "mxfp6_gemm.h"
+#include "route.hpp"
 
 namespace mxfp6 {
 
@@ -221,7 +222,7 @@ extern "C" int mxfp6_moe(const mxfp6_moe_layer* layer, int ot, int tokens, int t
     up.sB = pp.sx;
     up.n_entries = pp.n_entries;
     up.entries = pp.entries;
-    up.k_slabs = H / 128;
+    up.k_slabs = up.segment = H / 128;
     up.tiles = layer->gated ? I / 64 : I / 128;
     up.rows_per_expert = R1;
     up.inter = I;
@@ -236,6 +237,10 @@ extern "C" int mxfp6_moe(const mxfp6_moe_layer* layer, int ot, int tokens, int t
     down.sB = up.sh;
     down.k_slabs = I / 128;
     down.tiles = H / 128;
+    // An accumulator's error grows with the slabs it takes: an FP32 output's stay within FP32_SEGMENT_K (route.hpp). The hidden
+    // values and 16-bit outputs are rounded far more coarsely.
+    const int segments = ot == MXFP6_OUT_F32 ? (I + FP32_SEGMENT_K - 1) / FP32_SEGMENT_K : 1;
+    down.segment = (down.k_slabs + segments - 1) / segments;
     down.rows_per_expert = H;
     down.y = reinterpret_cast<float*>(b + w.y);
 
@@ -260,7 +265,9 @@ extern "C" int mxfp6_moe(const mxfp6_moe_layer* layer, int ot, int tokens, int t
     if (e == cudaSuccess)
         e = layer->gated ? launch_product_for<moe::KIND_UP_GATED>(w.nmax, tmW1, tmX, up, max_up, st)
                          : launch_product_for<moe::KIND_UP>(w.nmax, tmW1, tmX, up, max_up, st);
-    if (e == cudaSuccess) e = launch_product_for<moe::KIND_DOWN>(w.nmax, tmW2, tmH, down, max_down, st);
+    if (e == cudaSuccess)
+        e = segments > 1 ? launch_product_for<moe::KIND_DOWN_LONG>(w.nmax, tmW2, tmH, down, max_down, st)
+                         : launch_product_for<moe::KIND_DOWN>(w.nmax, tmW2, tmH, down, max_down, st);
     if (e == cudaSuccess) e = launch(moe::moe_combine, dim3((H + 1023) / 1024, tokens), 1, 256, 0, st, cp);
     if (e != cudaSuccess) {
         cudaGetLastError();

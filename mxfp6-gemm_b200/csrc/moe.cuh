@@ -423,6 +423,7 @@ struct ProductParams {
     const int* n_entries;
     const Entry* entries;
     int k_slabs;             // K / 128
+    int segment;             // down, long: slabs of one accumulator; an item's segments are added in FP32 in y
     int tiles;               // row tiles of one expert
     int rows_per_expert;     // rows of W per expert
     int inter, hidden, act;
@@ -435,16 +436,18 @@ struct ProductParams {
 // Cycles the abort path waits for copies and MMAs in flight (a quarter of the default wait budget).
 constexpr long long DRAIN_BUDGET = 1000000000LL;
 
-constexpr int KIND_UP_GATED = 0, KIND_UP = 1, KIND_DOWN = 2;
+// KIND_DOWN_LONG: a down product whose K is summed in segments, an accumulator each. It is an instantiation of its own because
+// the others took 1-4% longer with the segments' control flow.
+constexpr int KIND_UP_GATED = 0, KIND_UP = 1, KIND_DOWN = 2, KIND_DOWN_LONG = 3;
 
 template <int KIND, int NMAX>
 struct ProductConfig {
-    static constexpr bool GATED = KIND == KIND_UP_GATED;
+    static constexpr bool GATED = KIND == KIND_UP_GATED, DOWN = KIND >= KIND_DOWN, LONG = KIND == KIND_DOWN_LONG;
     static constexpr int A_BYTES = 128 * 128, B_BYTES = NMAX * 128, SF_BYTES = 1024;
     static constexpr int STAGE = A_BYTES + B_BYTES;
     static constexpr int CHUNK = NMAX < 32 ? NMAX : 32;  // tokens the epilogue takes at a time
     static constexpr int STG_PITCH = 132;
-    static constexpr int STG_BYTES = KIND == KIND_DOWN ? 0 : CHUNK * STG_PITCH * 4;
+    static constexpr int STG_BYTES = DOWN ? 0 : CHUNK * STG_PITCH * 4;
     static constexpr int BAR_BYTES = 256;
     static constexpr int CTAS = NMAX <= 64 ? 2 : 1;  // per SM
     static constexpr int BUDGET = (CTAS == 2 ? 113 : 226) * 1024 - 1024 - STG_BYTES - BAR_BYTES;
@@ -521,7 +524,7 @@ __global__ void __launch_bounds__(ProductConfig<KIND, NMAX>::THREADS, ProductCon
     // entries, and whatever wrote the weights, is complete. So the down product reads the list, and loads its first weight
     // tiles, while the up product still runs; its tokens (the hidden values) and outputs wait. Tokens go with the wait
     // in warp 0, outputs in warps 2..5.
-    constexpr bool EARLY = KIND == KIND_DOWN;
+    constexpr bool EARLY = C::DOWN;
     if (!EARLY) sm100::griddep_wait();
     // An entry, past L1: its lines are only sure to be newer than the list after the wait.
     auto entry = [&](int a) {
@@ -611,14 +614,29 @@ __global__ void __launch_bounds__(ProductConfig<KIND, NMAX>::THREADS, ProductCon
                 const int n = next.n;
                 next = entry_at(it + gridDim.x);
                 const uint32_t idesc = sm100::make_idesc_e2m3(128, (n + 15) / 16 * 16);
-                const int b = local & 1;
-                const uint32_t d_taddr = tmem_base + b * NMAX;
-                if (!sm100::wait_parity_bounded(acc_empty0 + 8u * b, ((local >> 1) & 1) ^ 1u, abort_flag, p.wait_budget)) {
-                    raise(0x2u);
-                    break;
-                }
-                sm100::tc_fence_after();
+                uint32_t d_taddr = 0;
+                auto next_accumulator = [&] {
+                    if (!sm100::wait_parity_bounded(acc_empty0 + 8u * (local & 1), ((local >> 1) & 1) ^ 1u, abort_flag,
+                                                    p.wait_budget)) {
+                        raise(0x2u);
+                        return false;
+                    }
+                    sm100::tc_fence_after();
+                    d_taddr = tmem_base + (local & 1) * NMAX;
+                    return true;
+                };
+                if (!next_accumulator()) break;
+                int kb0 = 0;  // the segment's first slab
                 for (int kb = 0; kb < p.k_slabs; kb++) {
+                    if (C::LONG && kb == kb0 + p.segment) {
+                        sm100::tc_commit(acc_full0 + 8u * (local & 1));
+                        local++;
+                        kb0 = kb;
+                        if (!next_accumulator()) {
+                            ok = false;
+                            break;
+                        }
+                    }
                     if (!ready && !sm100::wait_parity_bounded(full_bar(stage), phase, abort_flag, p.wait_budget)) {
                         raise(0x2u);
                         ok = false;
@@ -636,7 +654,7 @@ __global__ void __launch_bounds__(ProductConfig<KIND, NMAX>::THREADS, ProductCon
                                                sm100::make_kmajor_sw128_desc(b_src + 32 * k),
                                                sm100::idesc_with_sf_ids(idesc, k, k),
                                                (tmem_base + C::TMEM_SFA) | ((uint32_t)k << 30),
-                                               (tmem_base + C::TMEM_SFB) | ((uint32_t)k << 30), kb > 0 || k > 0 ? 1u : 0u);
+                                               (tmem_base + C::TMEM_SFB) | ((uint32_t)k << 30), kb > kb0 || k > 0 ? 1u : 0u);
                     mma_issued = true;
                     sm100::tc_commit(empty_bar(stage));
                     if (++stage == C::STAGES) {
@@ -645,17 +663,21 @@ __global__ void __launch_bounds__(ProductConfig<KIND, NMAX>::THREADS, ProductCon
                     }
                     ready = sm100::mbar_test_wait(full_bar(stage), phase);
                 }
-                if (ok) sm100::tc_commit(acc_full0 + 8u * b);
+                if (ok) sm100::tc_commit(acc_full0 + 8u * (local & 1));
             }
         }
     } else if (warp < 6) {
         const int quarter = warp & 3;
         int local = 0;
         Entry next = first;
-        for (int it = blockIdx.x; it < total; it += gridDim.x, local++) {
-            const int a = it / p.tiles, tile = it - a * p.tiles;
-            const Entry en = next;
-            next = entry_at(it + gridDim.x);
+        Entry en{};
+        int a = 0, tile = 0, kb0 = 0;  // kb0: the segment's first slab
+        for (int it = blockIdx.x; it < total; local++) {
+            if (!C::LONG || kb0 == 0) {
+                a = it / p.tiles, tile = it - a * p.tiles;
+                en = next;
+                next = entry_at(it + gridDim.x);
+            }
             const int b = local & 1;
             // all four warps leave together on a timeout (they share a barrier below)
             const bool got = sm100::wait_parity_bounded(acc_full0 + 8u * b, (local >> 1) & 1, abort_flag, p.wait_budget);
@@ -677,12 +699,13 @@ __global__ void __launch_bounds__(ProductConfig<KIND, NMAX>::THREADS, ProductCon
             for (int c0 = 0; c0 < en.n; c0 += C::CHUNK) {
                 uint32_t r[C::CHUNK];
                 sm100::tmem_ld_cols(t_acc + c0, r);
-                if constexpr (KIND == KIND_DOWN) {
+                if constexpr (C::DOWN) {
 #pragma unroll
                     for (int j = 0; j < C::CHUNK; j++)
-                        if (c0 + j < en.n)
-                            p.y[(size_t)(en.start + c0 + j) * p.hidden + tile * 128 + 32 * quarter + lane] =
-                                __uint_as_float(r[j]);
+                        if (c0 + j < en.n) {
+                            float* y = p.y + (size_t)(en.start + c0 + j) * p.hidden + tile * 128 + 32 * quarter + lane;
+                            *y = C::LONG && kb0 > 0 ? *y + __uint_as_float(r[j]) : __uint_as_float(r[j]);
+                        }
                 } else {
                     // token-major through shared memory: a thread then holds 16 hidden values of a token
 #pragma unroll
@@ -734,6 +757,8 @@ __global__ void __launch_bounds__(ProductConfig<KIND, NMAX>::THREADS, ProductCon
             }
             sm100::tc_fence_before();
             sm100::mbar_arrive(acc_empty0 + 8u * b);
+            if constexpr (C::LONG) kb0 = kb0 + p.segment < p.k_slabs ? kb0 + p.segment : 0;
+            if (!C::LONG || kb0 == 0) it += gridDim.x;
         }
     } else {
         // gated: rows 0..63 of a tile are gate rows, 64..127 up rows, so its scale atom takes 8 of the 16 bytes

@@ -364,3 +364,32 @@ def test_strides_of_tensors():
     torch.cuda.synchronize()
     assert lib.device_status() == 0 and (buf[:, 256:] == 9.0).all()
     check_rounded(buf[:, :256], *layer.reference(x, ids, w, res), ot)
+
+
+@pytest.mark.parametrize("inter", [12288, 14336, 28672, 57344])
+@pytest.mark.parametrize("T", [3, 40])
+def test_long_inter_in_fp32(inter, T):
+    """FP32 output of a long down product stays within the library's 1e-5. The up rows pick one value of x each, so the
+    hidden values are exact and nothing but the down product's sum is off."""
+    H = 128
+    W1 = np.zeros((inter, H), np.float32)
+    W1[np.arange(inter), np.arange(inter) % H] = 1.0
+    q = lib.quantize_to_mxfp6(W1)
+    W2 = Operand(H, inter, 1.0, 140)
+    raw = np.random.default_rng(142).integers(115, 135, (H, inter // 32)).astype(np.uint8)  # products of many magnitudes
+    W2.scales = torch.from_numpy(lib.preprocess_scale(raw, H, inter)).cuda()
+    W2.values = values(W2.packed.cpu().numpy(), raw, H, inter)
+    s1 = torch.from_numpy(lib.preprocess_scale(q.scales, inter, H)).cuda()
+    w1 = torch.from_numpy(q.packed_data).cuda()
+    layer = type("L", (), {"H": H, "layer": lib.MoELayer(1, H, inter, w1, s1, W2.packed, W2.scales, False, Act.NONE)})
+    x = _randn(T, H, seed=141)
+    ids, w = torch.zeros(T, 1, dtype=torch.int32, device="cuda"), torch.ones(T, 1, device="cuda")
+    qx = lib.quantize_to_mxfp6(x.cpu().numpy())
+    xv = values(qx.packed_data, qx.scales, T, H)
+    ref = xv.repeat(1, inter // H) @ W2.values.T
+    got = _moe(layer, OutType.F32, x, OutType.F32, 1, ids=ids, weights=w)
+    off = float((got.double() - ref).abs().max() / ref.abs().max())
+    assert off <= 1e-5, off
+    assert torch.equal(got, _moe(layer, OutType.F32, x, OutType.F32, 1, ids=ids, weights=w))
+    half = _moe(layer, OutType.BF16, x, OutType.F32, 1, ids=ids, weights=w)
+    check_rounded(half, ref, 1e-4 * ref.abs().max(), OutType.BF16)

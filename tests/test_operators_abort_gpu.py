@@ -59,3 +59,17 @@ def test_moe(gated):
     out = torch.empty(T, 4096, device="cuda")
     _expire(lambda: lib.moe(layer.layer, OutType.F32, T, k, x, OutType.BF16, out, ws, n, ids=ids, weights=w))
     check_rounded(_moe(layer, OutType.F32, x, OutType.BF16, k, ids=ids, weights=w), *layer.reference(x, ids, w), OutType.F32)
+
+
+def test_moe_long_inter():
+    """The down product in segments (FP32 output, inter above 12288)."""
+    layer = Layer(2, 1024, 24704)
+    T, k = 20, 1
+    x = _randn(T, 1024, seed=6, dtype=torch.bfloat16)
+    ids = torch.arange(T, device="cuda").view(T, 1).int() % 2
+    w = _randn(T, k, seed=7)
+    n = lib.moe_workspace_size(layer.layer, T, k)
+    ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+    out = torch.empty(T, 1024, device="cuda")
+    _expire(lambda: lib.moe(layer.layer, OutType.F32, T, k, x, OutType.BF16, out, ws, n, ids=ids, weights=w))
+    check_rounded(_moe(layer, OutType.F32, x, OutType.BF16, k, ids=ids, weights=w), *layer.reference(x, ids, w), OutType.F32)
