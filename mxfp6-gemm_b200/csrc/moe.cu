@@ -63,8 +63,10 @@ bool valid_layer(const mxfp6_moe_layer* l) {
            (long long)l->experts * l->hidden <= 0x7fffffff;
 }
 
-// Programmatic stream serialization: each kernel of the chain sets up while the one before it finishes, and
-// touches global memory only after griddepcontrol.wait.
+// Programmatic stream serialization: each kernel of the chain sets up while the one before it finishes. moe_prep and the up
+// product touch global memory only after griddepcontrol.wait. The down product reads the list of entries and its first weights
+// before its wait, and moe_combine the choices' places and weights before its own: both rest on moe_product letting its
+// dependents start only after its own wait, when moe_prep, and whatever wrote the weights, is complete.
 template <typename... KArgs, typename... Args>
 cudaError_t launch(void (*kernel)(KArgs...), dim3 grid, int cluster, int threads, size_t smem, cudaStream_t stream,
                    Args... args) {

@@ -535,6 +535,7 @@ __global__ void __launch_bounds__(ProductConfig<KIND, NMAX>::THREADS, ProductCon
     const Entry first = entry((int)blockIdx.x / p.tiles);
     const int total = sm100::ld_l2_s32(p.n_entries) * p.tiles;
     if (EARLY && warp != 0) sm100::griddep_wait();
+    // Never before this thread's wait (see moe.cu): the next kernel reads what moe_prep wrote without waiting for it.
     if (!EARLY || warp != 0) sm100::griddep_launch_dependents();
     // the entry of item `it`, read an item ahead of its use
     auto entry_at = [&](int it) { return it < total ? entry(it / p.tiles) : Entry{0, 0, 0, 0}; };
@@ -571,7 +572,7 @@ __global__ void __launch_bounds__(ProductConfig<KIND, NMAX>::THREADS, ProductCon
                         issued_mask |= 1u << kb;
                     }
                     sm100::griddep_wait();
-                    sm100::griddep_launch_dependents();
+                    sm100::griddep_launch_dependents();  // after the wait, as above
                 }
                 for (int kb = 0; kb < p.k_slabs; kb++) {
                     const uint32_t fb = full_bar(stage);
