@@ -233,8 +233,9 @@ inline Route route_for(int M, int N, int Kp, int sms, int min_splits = 1, bool f
 
 // Route of a fused GEMM of few rows (gemm_kernel_few.cuh): tile width and K segments, or splits == 0 where it does not
 // apply. One wave: the tiles of 128 columns times the segments fit two CTAs per SM, with room for the clusters that do
-// not fill a group of SMs (40 clusters of 7 on 148 SMs took two waves: 13.6 us against 8.6 us as clusters of 4). Wider
-// matrices take tiles of 256 columns, one per SM. Measured against the GEMM kernels with their split-K reduce (BF16, bias
+// not fill a group of SMs (40 clusters of 7 on 148 SMs took two waves: 13.6 us against 8.6 us as clusters of 4). Up to 16
+// rows a matrix that is only a little wider, so that one tile of 256 columns per SM still holds it (37377 to 37888 columns on
+// 148 SMs), takes those: 1 x 37632 x 4096 22.8 against 31.0 us, 16 x 37632 x 2048 15.5 against 17.4. Measured against the GEMM kernels with their split-K reduce (BF16, bias
 // and SiLU, back to back): 1 x 4096 x 4096 6.2 against 8.7 us, 16 x 8192 x 2048 6.9 / 9.1, 32 x 4096 x 4096 8.1 / 9.1,
 // 64 x 8192 x 2048 8.7 / 10.3, 128 x 4096 x 4096 13.1 / 10.8.
 //
@@ -253,7 +254,7 @@ inline Route few_route(int M, int N, int Kp, int sms, int min_splits) {
             return r;
         }
     r.NT = 256;
-    if (M <= 16 && wide <= sms && min_splits <= 1) r.splits = 1;  // 64 x 30000 x 2048: 22.4 against 19.0 us
+    if (M <= 16 && wide <= sms && min_splits <= 1) r.splits = 1;
     return r;
 }
 

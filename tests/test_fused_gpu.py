@@ -448,3 +448,35 @@ def test_activations_relative_error(M, N, K, act, low):
         off = (got[0].double() / ref - 1).abs()
         worst = (off - _activation_bound(act, x)).argmax()
         assert (off <= _activation_bound(act, x)).all(), (act, float(x[worst]), float(off[worst]))
+
+
+# Few rows of a matrix too wide for tiles of 128 columns at two per SM, and just narrow enough for tiles of 256 at one.
+@pytest.mark.parametrize("M,K", [(1, 1280), (3, 160), (16, 480)])
+def test_few_rows_of_wide_matrices(M, K):
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    first, last = (2 * sms - 4) * 128 + 1, sms * 256
+    A, B = Operand(M, K, 1.0, 90), Operand(last, K, K ** -0.5, 91)
+    whole = B.values
+    for N in (first, first + 6, last - 100, last):
+        B.rows, B.values = N, whole[:N]
+        bias = _randn(N, seed=92)
+        for ot, act, op in ((OutType.F32, Act.GELU, AuxOp.ADD), (OutType.BF16, Act.SILU, AuxOp.MUL), (OutType.F16, Act.NONE, AuxOp.NONE)):
+            aux = None if op == AuxOp.NONE else _randn(M, N, seed=93, dtype=DTYPE[ot])
+            got = _fused(A, B, ot, act, bias, aux=aux, aux_op=op, aux_type=ot)
+            check_rounded(got, *fused64(A, B, act, bias, aux, op), ot, f"{M}x{N}x{K}")
+
+
+@pytest.mark.parametrize("M", [1, 16])
+def test_few_rows_of_wide_matrices_quantised(M):
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    N, K = sms * 256 - 128, 640
+    A, B = Operand(M, K, 1.0, 94), Operand(N, K, K ** -0.5, 95)
+    bias = _randn(N, seed=96)
+    packed = torch.full((M + 1, N * 3 // 4), 0x5A, dtype=torch.uint8, device="cuda")
+    scales = torch.full((lib.tiled_scale_bytes(M, N),), 0x5A, dtype=torch.uint8, device="cuda")
+    assert lib.gemm_fused_quant(M, N, A.Kp, A.packed, B.packed, A.scales, B.scales, packed, scales, A.row_bytes, B.row_bytes,
+                                lib.Epilogue(bias, act=Act.SILU)) == lib.OK
+    _finish()
+    assert (packed[M] == 0x5A).all()
+    raw = lib.untile_scales(scales.cpu().numpy(), M, N)
+    check_quantised(packed[:M].cpu().numpy(), raw, *fused64(A, B, Act.SILU, bias, None, AuxOp.NONE), f"{M}x{N}")
