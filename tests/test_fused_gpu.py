@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import mxfp6_b200 as lib
-from fused_ref import DTYPE, Operand, act64, check_quantised, check_rounded, fused64
+from fused_ref import DTYPE, Operand, act64, check_quantised, check_rounded, fused64, values
 from mxfp6_b200 import Act, AuxOp, OutType
 
 pytestmark = pytest.mark.gpu
@@ -480,3 +480,61 @@ def test_few_rows_of_wide_matrices_quantised(M):
     assert (packed[M] == 0x5A).all()
     raw = lib.untile_scales(scales.cpu().numpy(), M, N)
     check_quantised(packed[:M].cpu().numpy(), raw, *fused64(A, B, Act.SILU, bias, None, AuxOp.NONE), f"{M}x{N}")
+
+
+@pytest.mark.parametrize("T,H,I", [(1, 256, 512), (19, 1024, 1408), (300, 512, 2048)])
+def test_gated_feed_forward_block(T, H, I):
+    """A gated block: the up half first, then the gate with it as the multiplied aux, to MXFP6, then the down product."""
+    Bg, Bu, Bd = Operand(I, H, H ** -0.5, 100), Operand(I, H, H ** -0.5, 101), Operand(H, I, I ** -0.5, 102)
+    x = _randn(T, H, seed=103, dtype=torch.bfloat16)
+    byte = lambda n: torch.zeros(n, dtype=torch.uint8, device="cuda")  # noqa: E731
+    n = max(lib.gemm_fused_workspace_size(T, I, H), lib.gemm_fused_workspace_size(T, H, I))
+    ws, xq, sx = byte(n), byte(T * H * 3 // 4), byte(lib.tiled_scale_bytes(T, H))
+    hq, sh = byte(T * I * 3 // 4), byte(lib.tiled_scale_bytes(T, I))
+    up, y = torch.empty(T, I, dtype=torch.bfloat16, device="cuda"), torch.empty(T, H, dtype=torch.bfloat16, device="cuda")
+    ot, rh, ri = OutType.BF16, H * 3 // 4, I * 3 // 4
+    gate, down = lib.Epilogue(act=Act.SILU, aux=up, aux_op=AuxOp.MUL), lib.Epilogue(aux=x, aux_op=AuxOp.ADD)
+    assert lib.quantize_device_typed(x, ot, T, H, H, H, xq, sx, tiled=True) == lib.OK
+    assert lib.gemm_fused(ot, T, I, H, xq, Bu.packed, sx, Bu.scales, up, rh, rh, None, ws, n) == lib.OK
+    assert lib.gemm_fused_quant(T, I, H, xq, Bg.packed, sx, Bg.scales, hq, sh, rh, rh, gate, ws, n) == lib.OK
+    assert lib.gemm_fused(ot, T, H, I, hq, Bd.packed, sh, Bd.scales, y, ri, ri, down, ws, n) == lib.OK
+    _finish()
+    q = lib.quantize_to_mxfp6(x.float().cpu().numpy())
+    A = type("A", (), {"values": values(q.packed_data, q.scales, T, H)})
+    check_rounded(up, *fused64(A, Bu, Act.NONE, None, None, AuxOp.NONE), ot, "up")
+    packed, raw = hq.cpu().numpy().reshape(T, -1), lib.untile_scales(sh.cpu().numpy(), T, I)
+    check_quantised(packed, raw, *fused64(A, Bg, Act.SILU, None, up, AuxOp.MUL), "hidden")
+    Hm = type("H", (), {"values": values(packed, raw, T, I)})
+    check_rounded(y, *fused64(Hm, Bd, Act.NONE, None, x, AuxOp.ADD), ot, "output")
+
+
+# D and aux of more than 2^31 elements: in place in the row layout, and the column layout.
+@pytest.mark.parametrize("N", [33024, 33023])
+def test_offsets_beyond_32_bits(N):
+    M, K = 66000, 128
+    A, B = Operand(M, K, 1.0, 110), Operand(N, K, K ** -0.5, 111)
+    D = torch.zeros(M, N, dtype=torch.bfloat16, device="cuda")
+    last = _randn(64, N, seed=112, dtype=torch.bfloat16)
+    D[-64:] = last
+    ep = lib.Epilogue(act=Act.RELU, aux=D, aux_op=AuxOp.ADD)
+    assert lib.gemm_fused(OutType.BF16, M, N, A.Kp, A.packed, B.packed, A.scales, B.scales, D, A.row_bytes, B.row_bytes, ep) == lib.OK
+    _finish()
+    for rows, aux in ((slice(0, 64), torch.zeros_like(last)), (slice(M - 64, M), last)):
+        part = type("A", (), {"values": A.values[rows]})
+        check_rounded(D[rows], *fused64(part, B, Act.RELU, None, aux, AuxOp.ADD), OutType.BF16, f"{N}")
+
+
+def test_quantiser_offsets_beyond_32_bits():
+    rows, cols = 66000, 33024
+    x = torch.zeros(rows, cols, dtype=torch.bfloat16, device="cuda")
+    x[-3:] = _randn(3, cols, seed=113, dtype=torch.bfloat16)
+    packed = torch.full((rows, cols * 3 // 4), 0x5A, dtype=torch.uint8, device="cuda")
+    scales = torch.full((lib.tiled_scale_bytes(rows, cols),), 0x5A, dtype=torch.uint8, device="cuda")
+    assert lib.quantize_device_typed(x, OutType.BF16, rows, cols, cols, cols, packed, scales, tiled=True) == lib.OK
+    torch.cuda.synchronize()
+    want = lib.quantize_to_mxfp6(x[-3:].float().cpu().numpy())
+    assert np.array_equal(packed[-3:].cpu().numpy(), want.packed_data) and (packed[:-3] == 0).all()
+    atoms = cols // 128 * 512  # bytes of a block of 128 rows
+    first = rows // 128 * 128
+    raw = lib.untile_scales(scales[-atoms:].cpu().numpy(), rows - first, cols)
+    assert np.array_equal(raw[-3:], want.scales) and (raw[:-3] == 127).all() and (scales[:-atoms] == 127).all()
