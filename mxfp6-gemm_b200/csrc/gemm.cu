@@ -957,16 +957,17 @@ void run_validated(int ot, int M, int N, int Kp, const void* dA, const void* dB,
         // the stream-K hand-off area takes 256-bit stores: a 256-byte aligned workspace
         if (!ws || ws_bytes < need || !aligned(ws, r.stream_k ? 256 : 16)) {
             // Same contract as the reference (src/dispatch.hpp:76-87): correct, only slower.
+            const char* query = fused ? "gemm_fused_workspace_size" : "gemm_workspace_size";
             if (r.splits > 1)
                 std::fprintf(stderr,
                              "[mxfp6] split-K skipped for %dx%dx%d: workspace %zu bytes, need %zu — "
-                             "running unsplit (slower). Size it with gemm_workspace_size().\n",
-                             M, N, Kp, ws_bytes, need);
+                             "running unsplit (slower). Size it with %s().\n",
+                             M, N, Kp, ws_bytes, need, query);
             else
                 std::fprintf(stderr,
                              "[mxfp6] stream-K tail skipped for %dx%dx%d: workspace %zu bytes (256-byte aligned), "
-                             "need %zu — running whole tiles (slower). Size it with gemm_workspace_size().\n",
-                             M, N, Kp, ws_bytes, need);
+                             "need %zu — running whole tiles (slower). Size it with %s().\n",
+                             M, N, Kp, ws_bytes, need, query);
             r.splits = 1;
             r.stream_k = false;
             r.banded = false;

@@ -538,3 +538,14 @@ def test_quantiser_offsets_beyond_32_bits():
     first = rows // 128 * 128
     raw = lib.untile_scales(scales[-atoms:].cpu().numpy(), rows - first, cols)
     assert np.array_equal(raw[-3:], want.scales) and (raw[:-3] == 127).all() and (scales[:-atoms] == 127).all()
+
+
+@pytest.mark.parametrize("M,N,K,what", [(100, 2560, 2048, "split-K"), (4090, 3570, 6144, "stream-K")])
+def test_skipped_workspace_names_the_query(capfd, M, N, K, what):
+    """A workspace of the size that the message's query gives is enough; gemm()'s own may not be."""
+    A, B = Operand(M, K, 1.0, 120), Operand(N, K, K ** -0.5, 121)
+    _fused(A, B, OutType.BF16, Act.SILU, ws=False)
+    err = capfd.readouterr().err
+    assert what in err and "gemm_fused_workspace_size()" in err
+    _fused(A, B, OutType.BF16, Act.SILU)
+    assert "skipped" not in capfd.readouterr().err
