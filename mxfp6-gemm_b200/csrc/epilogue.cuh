@@ -51,7 +51,8 @@ constexpr float LOG2E = 1.4426950408889634f;
 // The activations work on two values at a time. What bounds an exposed epilogue is the special-function unit (16 results
 // per clock and SM) about as much as issue slots: the packed arithmetic halves the latter, and two values share one
 // reciprocal (1.5 special-function results per value, not 2). 2048 x 6144 x 2048 with residual, FP16: GELU 37.1 -> 33.7
-// us, tanh GELU 36.7 -> 33.5, SiLU 34.6 -> 33.4; packed arithmetic with a reciprocal per value 35.1 / 35.6 / 34.8.
+// us (35.4 against 34.5 with the longer polynomial it has now), tanh GELU 36.7 -> 33.5, SiLU 34.6 -> 33.4; packed
+// arithmetic with a reciprocal per value 35.1 / 35.6 / 34.8.
 __device__ __forceinline__ F2 ex2(F2 x) {
     float a, b;
     split(x, a, b);
