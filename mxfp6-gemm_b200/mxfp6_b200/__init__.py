@@ -345,11 +345,13 @@ class Epilogue:
             _check_kind(what, t, kinds[-1])
         if hasattr(bias, "is_contiguous") and not bias.is_contiguous():
             raise ValueError("bias is not contiguous")
-        rows = _columns("aux", aux) and aux.dim() > 1 and aux.shape[0] > 1
+        strided = _columns("aux", aux)
         if ld_aux is None:
             if isinstance(aux, int):
                 raise ValueError("ld_aux is needed for an aux operand given as an address")
-            ld_aux = 0 if aux is None else aux.stride(0) if rows else aux.shape[-1]
+            if strided and aux.dim() > 2 and not aux.is_contiguous():
+                raise ValueError("ld_aux is needed for an aux tensor of more than two dimensions that is not contiguous")
+            ld_aux = 0 if aux is None else aux.stride(0) if strided and aux.dim() == 2 and aux.shape[0] > 1 else aux.shape[-1]
         self.keep = (bias, aux)
         self.struct = _EpilogueStruct(_addr(bias), _addr(aux), ld_aux, int(kinds[0]), int(act), int(aux_op), int(kinds[1]))
         self.ref = C.addressof(self.struct)

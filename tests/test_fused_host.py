@@ -139,3 +139,11 @@ def test_typed_quantiser_input_tensor(lib, torch, seen):
         with pytest.raises(ValueError):
             lib.quantize_device_typed(bad, t, 4, 64, 64, 64, P, P)
     assert len(seen) == 1
+
+
+def test_epilogue_aux_of_more_dimensions(lib, torch):
+    aux = torch.zeros(3, 4, 40)
+    assert lib.Epilogue(aux=aux).struct.ld_aux == 40  # [batch][token] rows
+    with pytest.raises(ValueError, match="ld_aux"):
+        lib.Epilogue(aux=aux[:, ::2])
+    assert lib.Epilogue(aux=aux[:, ::2], ld_aux=80).struct.ld_aux == 80
