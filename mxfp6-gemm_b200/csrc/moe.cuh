@@ -15,7 +15,8 @@
 //                holds both halves of each hidden value and quantises them) and down.
 //   moe_combine  the weighted sum over each token's choices, in their order.
 //
-// All FP32 sums are in tensor memory or registers, in a fixed order: results do not depend on timing.
+// All FP32 sums are in tensor memory or registers, in a fixed order (a long down product's segments in y, by the thread that
+// wrote them): results do not depend on timing.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
